@@ -25,7 +25,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // Epilogue arithmetic.  The epilogues run between two barriers with the matrix pipe idle and are VALU-bound (64
-// accumulator values per lane and stage), so every value is kept to ~6 instructions: packed fp32 fma / mul, packed
+// accumulator values per lane and stage), so every value is kept to ~6 instructions: fp32 fma / mul, packed
 // conversions, and the low part by ONE mixed-precision fma per value that reads the fp16 high part directly,
 //     lo = f16( hi * -2^11 + v * 2^11 )          (v_fma_mixlo/hi_f16: exact fp32 fma, one rounding to fp16)
 // which is bit-identical to f16((v - f32(hi)) * 2^11): the difference and both scalings are exact.

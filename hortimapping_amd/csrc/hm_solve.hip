@@ -320,7 +320,7 @@ __device__ bool pcg_solve(const float* __restrict__ H, int ld, const float* diag
   // 4 (j + 16 c) .. + 3, c = 0..3, of row 4 g + r (conflict-free 16-byte reads: consecutive lanes, consecutive float4s).
   // The row dot products then reduce INSIDE a DPP row (four v_add_dpp, no cross-row traffic, all four rows at once);
   // the column sums stay in 16 registers per lane and are merged across DPP rows (lane swaps) / waves (LDS, fixed order)
-  // once per mat-vec.  Packed fp32 FMAs (v_pk_fma_f32) halve the instruction count of the products.
+  // once per mat-vec. 
   const int dr = lane >> 4, dj = lane & 15;
   bool conv = false;
   for (int it = 0; it < CG_MAXIT; ++it) {
