@@ -20,6 +20,15 @@ class HortiHipError(RuntimeError):
     pass
 
 
+class HmAdapterArgs(ctypes.Structure):
+    """ctypes mirror of `hm_adapter_args` (include/hortimapping_amd.h)."""
+    _fields_ = [("type", c_int), ("k", c_int), ("n", c_int), ("rank", c_int), ("adapters", c_int), ("segments", c_int),
+                ("tag", ctypes.c_uint), ("rows", ctypes.c_longlong), ("d_x", c_void_p), ("ld_x", ctypes.c_longlong),
+                ("d_w", c_void_p), ("ld_w", ctypes.c_longlong), ("d_bias", c_void_p), ("d_a", c_void_p), ("d_b", c_void_p),
+                ("d_scale", c_void_p), ("d_row_start", c_void_p), ("d_adapter", c_void_p), ("p", ctypes.c_double),
+                ("seed", ctypes.c_ulonglong), ("d_seed", c_void_p), ("row0", ctypes.c_ulonglong)]
+
+
 def _declare(lib):
     lib.hm_last_error.restype = ctypes.c_char_p
     lib.hm_last_error.argtypes = []
@@ -41,6 +50,21 @@ def _declare(lib):
     lib.hm_decode_batch.restype = c_int
     lib.hm_decode_batch.argtypes = [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p,
                                     c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]
+    ll, ull, dbl = ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_double
+    lib.hm_dropout.restype = c_int
+    lib.hm_dropout.argtypes = [c_void_p, ll, c_void_p, ll, ll, c_int, c_int, c_int, dbl, ull, c_void_p, ctypes.c_uint, ull,
+                               c_void_p]
+    lib.hm_dropout_backward.restype = c_int
+    lib.hm_dropout_backward.argtypes = [c_void_p, ll, c_void_p, ll, c_void_p, ll, ll, c_int, c_int, c_int, dbl, ull, c_void_p,
+                                        ctypes.c_uint, ull, c_void_p]
+    args_p = ctypes.POINTER(HmAdapterArgs)
+    lib.hm_adapter_linear.restype = c_int
+    lib.hm_adapter_linear.argtypes = [args_p, c_void_p, ll, c_void_p, c_void_p]
+    lib.hm_adapter_linear_backward_bytes.restype = ll
+    lib.hm_adapter_linear_backward_bytes.argtypes = [args_p]
+    lib.hm_adapter_linear_backward.restype = c_int
+    lib.hm_adapter_linear_backward.argtypes = [args_p, c_void_p, ll, c_void_p, c_void_p, ll, c_void_p, c_void_p, c_void_p, ll,
+                                               c_void_p]
 
 
 def lib():

@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "..", "build", "obj")
 LIB = os.path.join(HERE, "libhortihip.so")
 SOURCES = ["hm_pack.hip", "hm_decoder.hip", "hm_decoder_h.hip", "hm_decoder_p.hip", "hm_decoder_any.hip", "hm_normal_eq.hip", "hm_solve.hip", "hm_render.hip",
-           "hm_optimize.hip", "hm_mesh.hip", "hm_metrics.hip", "hm_prep.hip", "hm_debug.hip", "hm_api.hip"]
+           "hm_optimize.hip", "hm_mesh.hip", "hm_metrics.hip", "hm_dropout.hip", "hm_adapter.hip", "hm_prep.hip", "hm_debug.hip", "hm_api.hip"]
 # Packed fp32 instructions are switched off: some of their forms have given wrong results on MI355X now and then, without an
 # error.  (The host pass of hipcc warns that it does not know the feature: harmless.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -1,0 +1,873 @@
+// Low-rank adapters of many requests at once beside a shared projection (LoRA-style fine-tuning and serving of ONE decoder
+// for many species / cultivars; the projection is one Linear of deepsdf/networks/deep_sdf_decoder.py:29-62):
+//
+//   y[m]  = x[m] W^T + b + t[m] B_a^T            t[m] = s_a drop(x[m]) A_a^T      a = adapter of the request that row m is in
+//   dx[m] = dy[m] W + drop'(u[m] A_a)            u[m] = s_a dy[m] B_a
+//   dA_a  = sum_m u[m]^T drop(x[m])              dB_a = sum_m dy[m]^T t[m]        (the projection is frozen)
+//
+// x (M, K), W (N, K), A (adapters, r, K), B (adapters, N, r).  Request q has the rows row_start[q] .. row_start[q + 1] - 1 and
+// the adapter adapter[q]; a value outside 0 .. adapters - 1, or no request at all, leaves the bare projection.
+//
+// Arithmetic: every sum is held in 32 bits.  t and u stay in 32 bits in memory; where they meet 16-bit weights on the matrix
+// cores they are split into a high and a low 16-bit part (two products: the rank is small), so they add no rounding.  A value
+// kept by the dropout is NOT multiplied by 1 / (1 - p) before the product (that would round it): the factor joins s_a.
+// fp16: |t| or |u| beyond 65504 overflows to infinity.
+//
+// A row's result depends on its own row and its own adapter alone: a lane of a matrix product holds one row (rows are the
+// columns of the MFMA), and what another request's adapter adds is selected away, not multiplied by 0 -- an infinity or NaN in
+// one request or one adapter does not reach another request.  Sums over rows (dA, dB) run in a fixed order: no atomics.
+#include "hm_internal.h"
+#include "hm_keep.h"
+#include "../../include/hortimapping_amd.h"
+
+using namespace hm;
+
+namespace {
+
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+struct Segs {
+  const int* row_start;   // [S + 1]
+  const int* adapter;     // [S]
+  const float* scale;     // [adapters] or nullptr
+  int S, n_adapters, M;
+};
+
+// last request that starts at or before `row` (-1: none), found by the whole wave: 64 probes a step.  Whatever row_start
+// holds, the result is in -1 .. S - 1.
+__device__ __forceinline__ int seg_find(const Segs& sg, int row) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = sg.S;
+  while (n > 0) {
+    const int step = (n + 63) >> 6, at = lo + lane * step;
+    const bool le = lane * step < n && sg.row_start[at] <= row;
+    const int c = __popcll(__ballot(le));
+    if (c == 0) return lo - 1;
+    lo += (c - 1) * step;
+    if (step == 1) return lo;
+    const int left = n - (c - 1) * step;
+    n = left < step ? left : step;
+  }
+  return -1;
+}
+
+// the rows of request q inside [r0, r1), and its adapter (-1: none of them)
+struct Span { int lo, hi, a; };
+__device__ __forceinline__ Span seg_span(const Segs& sg, int q, int r0, int r1) {
+  const int s0 = sg.row_start[q], s1 = sg.row_start[q + 1], a = sg.adapter[q];
+  Span s = {s0 > r0 ? s0 : r0, s1 < r1 ? s1 : r1, a};
+  if (a < 0 || a >= sg.n_adapters || s.lo >= s.hi) s.a = -1;
+  return s;
+}
+
+// ---- fragments of eight consecutive values along the reduction, and 16 x 16 products over 32 of it
+template <typename T> struct Frag8;
+template <> struct Frag8<float> { float v[8]; };
+template <> struct Frag8<f16> { f16x8 v; };
+template <> struct Frag8<bf16> { bf16x8 v; };
+
+__device__ __forceinline__ f32x4 mma16(const Frag8<f16>& a, const Frag8<f16>& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(const Frag8<bf16>& a, const Frag8<bf16>& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(const Frag8<float>& a, const Frag8<float>& b, f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
+  return c;
+}
+
+// p[0 .. 7], of which the first n exist (n <= 0: none): zero where nothing is
+template <typename T> __device__ __forceinline__ Frag8<T> frag_load(const T* p, int n) {
+  Frag8<T> f;
+  if (n >= 8) {
+    const Pack8<T> u = *reinterpret_cast<const Pack8<T>*>(p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.v[j] = u.v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.v[j] = j < n ? p[j] : (T)0.f;
+  }
+  return f;
+}
+template <typename T> __device__ __forceinline__ void frag_keep(Frag8<T>& f, uint32_t keep) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f.v[j] = (keep >> j) & 1 ? f.v[j] : (T)0.f;
+}
+
+// ---- t / u: 32 rows x up to 64 ranks per workgroup, the four waves share the reduction.  Bound by reading X once.
+constexpr int SH_ROWS = 32, SH_RANKS = 64;
+
+template <typename T, int RT, bool DROP>
+__global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ R, long long ldr,
+                                                long long stride_a, int rank, float factor, Segs sg, KeepArgs ka,
+                                                float* __restrict__ t) {
+  __shared__ f32x4 red[4][2 * RT][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+  const int r0 = blockIdx.x * SH_ROWS, ib = blockIdx.y * SH_RANKS;
+  const int r1 = r0 + SH_ROWS < sg.M ? r0 + SH_ROWS : sg.M;
+  const KeepKey key = keep_key(ka);
+  const int steps = (K + 31) >> 5;
+  int q = seg_find(sg, r0);
+  for (q = q < 0 ? 0 : q; q < sg.S && sg.row_start[q] < r1; ++q) {
+    const Span sp = seg_span(sg, q, r0, r1);
+    if (sp.a < 0) continue;
+    f32x4 acc[2][RT];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int i = 0; i < RT; ++i) acc[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const T* Ra = R + (long long)sp.a * stride_a;
+    for (int s = w; s < steps; s += 4) {
+      const int k = 32 * s + 8 * g, n = K - k;
+      Frag8<T> x[2], a[RT];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int row = r0 + 16 * m + l16;
+        x[m] = frag_load(X + row * ldx + k, row < sg.M ? n : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int ri = ib + 16 * i + l16;
+        a[i] = frag_load(Ra + ri * ldr + k, ri < rank ? n : 0);
+      }
+      if (DROP) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) frag_keep(x[m], keep8(ka, key, (uint64_t)(r0 + 16 * m + l16), (uint32_t)(k >> 3)));
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[m][i] = mma16(a[i], x[m], acc[m][i]);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int i = 0; i < RT; ++i) red[w][m * RT + i][lane] = acc[m][i];
+    __syncthreads();
+    const float f = factor * (sg.scale != nullptr ? sg.scale[sp.a] : 1.f);
+#pragma unroll
+    for (int v4 = 0; v4 < (2 * RT + 3) / 4; ++v4) {
+      const int u = w + 4 * v4;
+      if (u >= 2 * RT) break;
+      const f32x4 v = (red[0][u][lane] + red[1][u][lane]) + (red[2][u][lane] + red[3][u][lane]);
+      const int row = r0 + 16 * (u / RT) + l16, i0 = ib + 16 * (u % RT) + 4 * g;
+      if (row >= sp.lo && row < sp.hi) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i0 + j < rank) t[(long long)row * rank + i0 + j] = v[j] * f;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// the same for requests of few rows (single tokens): a wave takes one row and four ranks, its lanes the reduction
+constexpr int SR_RANKS = 4;
+
+template <typename T, bool DROP>
+__global__ __launch_bounds__(256) void k_shrink_rows(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ R, long long ldr,
+                                                     long long stride_a, int rank, float factor, Segs sg, KeepArgs ka,
+                                                     float* __restrict__ t) {
+  const int lane = threadIdx.x & 63, groups = (rank + SR_RANKS - 1) / SR_RANKS;
+  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int row = (int)(id / groups), i0 = (int)(id % groups) * SR_RANKS;
+  if (row >= sg.M) return;
+  const int q = seg_find(sg, row);
+  if (q < 0) return;
+  const Span sp = seg_span(sg, q, row, row + 1);
+  if (sp.a < 0) return;
+  const KeepKey key = keep_key(ka);
+  const T* Ra = R + (long long)sp.a * stride_a;
+  float acc[SR_RANKS] = {};
+  for (int k = 8 * lane; k < K; k += 512) {
+    Frag8<T> x = frag_load(X + row * ldx + k, K - k);
+    if (DROP) frag_keep(x, keep8(ka, key, (uint64_t)row, (uint32_t)(k >> 3)));
+#pragma unroll
+    for (int i = 0; i < SR_RANKS; ++i) {
+      const Frag8<T> a = frag_load(Ra + (i0 + i) * ldr + k, i0 + i < rank ? K - k : 0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i] = fmaf((float)x.v[j], (float)a.v[j], acc[i]);
+    }
+  }
+  const float f = factor * (sg.scale != nullptr ? sg.scale[sp.a] : 1.f);
+#pragma unroll
+  for (int i = 0; i < SR_RANKS; ++i) {
+    float v = acc[i];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    if (lane == i && i0 + i < rank) t[(long long)row * rank + i0 + i] = v * f;
+  }
+}
+
+// ---- the projection with the low-rank part: out (M, Nn) = X (M, Kk) W^T (+ bias) + t Bt_a^T, tiles of BM x BN in LDS, rows of
+// 128 bytes along the reduction, 16-byte chunks XOR-ed with the row (conflict-free 16-byte reads)
+template <typename T> struct Lines { static constexpr int V = 16 / sizeof(T), KB = 128 / sizeof(T); };
+template <typename T> struct alignas(16) Line { T v[16 / sizeof(T)]; };
+
+__device__ __forceinline__ f32x16 mma32(uint4 a, uint4 b, f32x16 c, f16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(uint4 a, uint4 b, f32x16 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(uint4 a, uint4 b, f32x16 c, float) {
+  const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+  return c;
+}
+
+template <typename T> __device__ __forceinline__ uint4 line_load(const T* p, int n) {
+  constexpr int V = Lines<T>::V;
+  struct alignas(sizeof(T)) P { T v[V]; };
+  Line<T> o;
+  if (n >= V) {
+    const P u = *reinterpret_cast<const P*>(p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.v[j] = u.v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.v[j] = j < n ? p[j] : (T)0.f;
+  }
+  return __builtin_bit_cast(uint4, o);
+}
+
+struct LowRank {
+  const float* t;          // [M][rank], or nullptr: no adapters at all
+  const void* b;           // element (adapter a, output n, i) at a * sa + n * sn + i * si
+  long long sa, sn, si;
+  int rank;
+};
+
+template <typename T, int BM, int BN, int WGM, int WGN, bool DROP>
+__global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict__ X, long long ldx, int Kk, const T* __restrict__ W,
+                                                            long long ldw, int Nn, const T* __restrict__ bias, LowRank lr, Segs sg,
+                                                            KeepArgs ka, T* __restrict__ out, long long ldo, int tiles_n) {
+  constexpr int NT = 64 * WGM * WGN, MI = BM / WGM / 32, NI = BN / WGN / 32, V = Lines<T>::V, KB = Lines<T>::KB;
+  constexpr int RX = BM * 8 / NT, RW = BN * 8 / NT;
+  __shared__ uint4 sx[2][BM * 8], sw[2][BN * 8];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w % WGM, wn = w / WGM, l32 = lane & 31, h = lane >> 5;
+  // consecutive workgroups go to the eight XCDs in turn: give each XCD a contiguous run of tiles, so that the tiles that share
+  // rows of X share an L2
+  const int total = gridDim.x, xcd = blockIdx.x & 7, per = total >> 3, extra = total & 7;
+  const int tile = xcd * per + (xcd < extra ? xcd : extra) + (blockIdx.x >> 3);
+  const int m0 = (tile / tiles_n) * BM, n0 = (tile % tiles_n) * BN;
+  const int m1 = m0 + BM < sg.M ? m0 + BM : sg.M;
+  f32x16 acc[NI][MI];
+#pragma unroll
+  for (int n = 0; n < NI; ++n)
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[n][m][j] = 0.f;
+
+  if (lr.t != nullptr) {
+    const T* b = static_cast<const T*>(lr.b);
+    int q = seg_find(sg, m0);
+    for (q = q < 0 ? 0 : q; q < sg.S && sg.row_start[q] < m1; ++q) {
+      const Span sp = seg_span(sg, q, m0, m1);
+      if (sp.a < 0) continue;
+      const T* ba = b + (long long)sp.a * lr.sa;
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const int row = m0 + (wm * MI + m) * 32 + l32;
+        const bool mine = row >= sp.lo && row < sp.hi;
+        if (__ballot(mine) == 0) continue;
+        const float* tr = lr.t + (long long)(mine ? row : sp.lo) * lr.rank;
+        f32x16 add[NI];
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) add[n][j] = 0.f;
+        for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
+          const int i = i0 + V * h;
+          Line<T> hi, lo;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float v = i + j < lr.rank ? tr[i + j] : 0.f;
+            hi.v[j] = (T)v;
+            const float f = (float)hi.v[j];
+            lo.v[j] = (T)(fabsf(f) < INFINITY ? v - f : 0.f);
+          }
+#pragma unroll
+          for (int n = 0; n < NI; ++n) {
+            const int col = n0 + (wn * NI + n) * 32 + l32;
+            Line<T> b8;
+#pragma unroll
+            for (int j = 0; j < V; ++j) b8.v[j] = col < Nn && i + j < lr.rank ? ba[col * lr.sn + (i + j) * lr.si] : (T)0.f;
+            const uint4 bf = __builtin_bit_cast(uint4, b8);
+            add[n] = mma32(bf, __builtin_bit_cast(uint4, hi), add[n], T());
+            if (sizeof(T) == 2) add[n] = mma32(bf, __builtin_bit_cast(uint4, lo), add[n], T());
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[n][m][j] = mine ? add[n][j] : acc[n][m][j];
+      }
+    }
+    if (DROP) {                                       // the mask of x on the low-rank part of dx
+      const KeepKey key = keep_key(ka);
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const int row = m0 + (wm * MI + m) * 32 + l32;
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+          const int cb = (n0 + (wn * NI + n) * 32) >> 3;
+          // lane h makes the draws of column blocks 2 h and 2 h + 1; its partner holds the other half of each block's columns
+          const uint32_t k2 = keep8(ka, key, (uint64_t)row, cb + 2 * h) | keep8(ka, key, (uint64_t)row, cb + 2 * h + 1) << 8;
+          const uint32_t o2 = __shfl_xor(k2, 32);
+          const uint32_t k4 = h == 0 ? (k2 | o2 << 16) : (o2 | k2 << 16);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            acc[n][m][j] = (k4 >> (8 * (j >> 2) + 4 * h + (j & 3))) & 1 ? acc[n][m][j] * ka.up : 0.f;
+        }
+      }
+    }
+  }
+
+  const int c = tid & 7, rr = tid >> 3;
+  uint4 gx[RX], gw[RW];
+  const int steps = (Kk + KB - 1) / KB;
+  auto fetch = [&](int s) {
+    const int k = s * KB + c * V, n = Kk - k;
+#pragma unroll
+    for (int j = 0; j < RX; ++j) {
+      const int row = m0 + rr + j * (NT / 8);
+      gx[j] = line_load(X + row * ldx + k, row < sg.M ? n : 0);
+    }
+#pragma unroll
+    for (int j = 0; j < RW; ++j) {
+      const int row = n0 + rr + j * (NT / 8);
+      gw[j] = line_load(W + row * ldw + k, row < Nn ? n : 0);
+    }
+  };
+  auto stash = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < RX; ++j) { const int r = rr + j * (NT / 8); sx[buf][r * 8 + (c ^ (r & 7))] = gx[j]; }
+#pragma unroll
+    for (int j = 0; j < RW; ++j) { const int r = rr + j * (NT / 8); sw[buf][r * 8 + (c ^ (r & 7))] = gw[j]; }
+  };
+  if (steps > 0) {
+    fetch(0);
+    stash(0);
+    if (steps > 1) fetch(1);
+    __syncthreads();
+  }
+  for (int s = 0; s < steps; ++s) {
+    const int buf = s & 1;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      uint4 fx[MI], fw[NI];
+#pragma unroll
+      for (int m = 0; m < MI; ++m) { const int r = (wm * MI + m) * 32 + l32; fx[m] = sx[buf][r * 8 + ((2 * kk + h) ^ (r & 7))]; }
+#pragma unroll
+      for (int n = 0; n < NI; ++n) { const int r = (wn * NI + n) * 32 + l32; fw[n] = sw[buf][r * 8 + ((2 * kk + h) ^ (r & 7))]; }
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+#pragma unroll
+        for (int m = 0; m < MI; ++m) acc[n][m] = mma32(fw[n], fx[m], acc[n][m], T());
+    }
+    if (s + 1 < steps) {
+      stash(buf ^ 1);
+      if (s + 2 < steps) fetch(s + 2);
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int n = 0; n < NI; ++n) {
+    const int cb = n0 + (wn * NI + n) * 32;
+#pragma unroll
+    for (int j4 = 0; j4 < 4; ++j4) {
+      const int col = cb + 8 * j4 + 4 * h;
+      float bv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bv[j] = bias != nullptr && col + j < Nn ? (float)bias[col + j] : 0.f;
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const int row = m0 + (wm * MI + m) * 32 + l32;
+        if (row >= sg.M) continue;
+        T* o = out + row * ldo + col;
+        struct alignas(sizeof(T)) P { T v[4]; } p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p.v[j] = (T)(acc[n][m][4 * j4 + j] + bv[j]);
+        if (col + 4 <= Nn) {
+          *reinterpret_cast<P*>(o) = p;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) if (col + j < Nn) o[j] = p.v[j];
+        }
+      }
+    }
+  }
+}
+
+// ---- few rows (M <= 64): the weights are read once, sixteen outputs a workgroup, its waves share the reduction
+constexpr int FEW_ROWS = 64, FEW_WAVES = 8;
+
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ W,
+                                                                long long ldw, int N, const T* __restrict__ bias, LowRank lr, Segs sg,
+                                                                T* __restrict__ out, long long ldo) {
+  __shared__ f32x4 red[FEW_WAVES][MT][64];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16, steps = (K + 31) >> 5;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = w; s < steps; s += FEW_WAVES) {
+    const int k = 32 * s + 8 * g, n = K - k;
+    const Frag8<T> a = frag_load(W + (n0 + l16) * ldw + k, n0 + l16 < N ? n : 0);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = 16 * m + l16;
+      acc[m] = mma16(a, frag_load(X + row * ldx + k, row < sg.M ? n : 0), acc[m]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) red[w][m][lane] = acc[m];
+  __syncthreads();
+  if (w >= MT) return;
+  f32x4 v = red[0][w][lane];
+#pragma unroll
+  for (int u = 1; u < FEW_WAVES; ++u) v += red[u][w][lane];
+  // lane: row 16 w + l16, outputs n0 + 4 g .. + 3
+  const int row = 16 * w + l16, col = n0 + 4 * g;
+  int a = -1;
+  if (lr.t != nullptr && row < sg.M) {
+    int lo = 0, hi = sg.S;                             // last request that starts at or before the row
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (sg.row_start[mid] <= row) lo = mid + 1; else hi = mid; }
+    if (lo > 0) a = seg_span(sg, lo - 1, row, row + 1).a;
+  }
+  if (a >= 0) {
+    const T* b = static_cast<const T*>(lr.b) + (long long)a * lr.sa;
+    for (int i = 0; i < lr.rank; ++i) {
+      const float ti = lr.t[(long long)row * lr.rank + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < N) v[j] = fmaf(ti, (float)b[(col + j) * lr.sn + i * lr.si], v[j]);
+    }
+  }
+  if (row < sg.M) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < N) out[row * ldo + col + j] = (T)(v[j] + (bias != nullptr ? (float)bias[col + j] : 0.f));
+  }
+}
+
+// ---- sums over rows: G_a[p][i] = sum over the rows m of adapter a of X[m][p] t[m][i], 128 columns p and up to 64 ranks a
+// workgroup.  The reduction runs along the rows, so both operands are read as they lie: 16 x 16 x 4 fp32 products, lane (p, m).
+// The fp32 matrix rate is above what reading X needs up to a rank of 16 and keeps t exact.
+constexpr int OU_COLS = 128;
+
+// adds rows [lo, hi) to the sums of the four waves: wave w takes four rows of every sixteen
+template <typename T, int RT>
+__device__ __forceinline__ void outer_rows(f32x4 (&acc)[8][RT], const T* X, long long ldx, int P, const float* t, int rank, int ib,
+                                           int p, int lo, int hi, int w, int lane, bool drop, const KeepArgs& ka, KeepKey key) {
+  const int l16 = lane & 15, g = lane >> 4;
+  for (int m0 = lo + 4 * w; m0 < hi; m0 += 16) {
+    const int m = m0 + g;
+    const bool in = m < hi;
+    Frag8<T> x = frag_load(X + (long long)(in ? m : lo) * ldx + p, in ? P - p : 0);
+    if (drop) frag_keep(x, keep8(ka, key, (uint64_t)m, (uint32_t)(p >> 3)));
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int ri = ib + 16 * i + l16;
+      const float tv = in && ri < rank ? t[(long long)m * rank + ri] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[j], tv, acc[j][i], 0, 0, 0);
+    }
+  }
+}
+
+// one job of the sums: dA (X = x, t = u) or dB (X = dy, t = t)
+struct Outer {
+  const void* X;
+  long long ldx;
+  int P;                   // columns
+  const float* t;
+  void* out;               // element (a, p, i) at a * oa + p * op + i * oi
+  long long oa, op, oi;
+  float* part;             // [slot][column block][rank chunk][tile (j, i)][lane] f32x4
+  int blocks;              // column blocks
+  int drop;
+  float factor;
+};
+
+template <int RT> __device__ __forceinline__ size_t part_at(const Outer& o, int slot, int pb, int rc, int chunks) {
+  return (((size_t)slot * o.blocks + pb) * chunks + rc) * (8 * RT * 64);
+}
+
+// value q of tile (j, i) in `lane`: column pb * 128 + 8 (4 (lane / 16) + q) + j, rank ib + 16 i + lane % 16
+template <typename T, int RT>
+__device__ __forceinline__ void outer_store(const Outer& o, f32x4 v, int tile, int lane, int a, int pb, int ib, int rank) {
+  const int j = tile / RT, i = ib + 16 * (tile % RT) + (lane & 15);
+  if (i >= rank) return;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int p = pb * OU_COLS + 8 * (4 * (lane >> 4) + q) + j;
+    if (p < o.P) static_cast<T*>(o.out)[a * o.oa + p * o.op + i * o.oi] = (T)(v[q] * o.factor);
+  }
+}
+
+// partial sums of a run of rows, one slot for each (run, request) pair: run + request numbers it, for a step to the next pair
+// raises one of the two
+template <typename T, int RT>
+__device__ __forceinline__ void outer_run(const Outer& o, const Segs& sg, const KeepArgs& ka, int rank, int rows_per_run, f32x4 (*red)[8][64]) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15;
+  const int pb = blockIdx.x, run = blockIdx.y, chunks = (rank + 63) / 64;
+  const int r0 = run * rows_per_run, r1 = sg.M - r0 < rows_per_run ? sg.M : r0 + rows_per_run;
+  const KeepKey key = keep_key(ka);
+  int q = seg_find(sg, r0);
+  for (q = q < 0 ? 0 : q; q < sg.S && sg.row_start[q] < r1; ++q) {
+    const Span sp = seg_span(sg, q, r0, r1);
+    if (sp.a < 0) continue;
+    for (int rc = 0; rc < chunks; ++rc) {
+      f32x4 acc[8][RT];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      outer_rows<T, RT>(acc, static_cast<const T*>(o.X), o.ldx, o.P, o.t, rank, 64 * rc, pb * OU_COLS + 8 * l16, sp.lo, sp.hi, w, lane, o.drop != 0, ka, key);
+      f32x4* to = reinterpret_cast<f32x4*>(o.part) + part_at<RT>(o, run + q, pb, rc, chunks);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) red[w][j][lane] = acc[j][i];
+        __syncthreads();
+        for (int j = w; j < 8; j += 4)
+          to[(j * RT + i) * 64 + lane] = (red[0][j][lane] + red[1][j][lane]) + (red[2][j][lane] + red[3][j][lane]);
+        __syncthreads();
+      }
+    }
+  }
+}
+
+template <typename T, int RT>
+__global__ __launch_bounds__(256) void k_outer(Outer oa, Outer ob, Segs sg, KeepArgs ka, int rank, int rows_per_run) {
+  __shared__ f32x4 red[4][8][64];
+  const Outer& o = blockIdx.z == 0 ? oa : ob;
+  if ((int)blockIdx.x >= o.blocks) return;
+  outer_run<T, RT>(o, sg, ka, rank, rows_per_run, red);
+}
+
+// requests of an adapter in ascending order, 256 looked at a time
+struct ReqList { int n; int q[256]; };
+__device__ __forceinline__ void list_requests(const Segs& sg, int a, int base, ReqList* l) {
+  __shared__ int cnt[4];
+  const int q = base + threadIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const bool is = q < sg.S && sg.adapter[q] == a && sg.row_start[q] < sg.row_start[q + 1];
+  const unsigned long long b = __ballot(is);
+  __syncthreads();                                     // the list of the last step is read
+  if (lane == 0) cnt[w] = __popcll(b);
+  __syncthreads();
+  int at = 0;
+  for (int i = 0; i < w; ++i) at += cnt[i];
+  if (is) l->q[at + __popcll(b & ((1ull << lane) - 1))] = q;
+  if (threadIdx.x == 0) l->n = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+  __syncthreads();
+}
+
+// sums the slots of an adapter, in order of requests and runs
+template <typename T, int RT>
+__global__ __launch_bounds__(256) void k_outer_sum(Outer oa, Outer ob, Segs sg, int rank, int rows_per_run) {
+  __shared__ ReqList list;
+  const Outer& o = blockIdx.z == 0 ? oa : ob;
+  const int chunks = (rank + 63) / 64, parts = 8 * RT / 4;      // four tiles a workgroup
+  const int a = blockIdx.y, per = o.blocks * chunks * parts;
+  if ((int)blockIdx.x >= per) return;
+  const int pb = blockIdx.x / (chunks * parts), rc = blockIdx.x / parts % chunks, tile = blockIdx.x % parts * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int base = 0; base < sg.S; base += 256) {
+    list_requests(sg, a, base, &list);
+    for (int e = 0; e < list.n; ++e) {
+      const int q = list.q[e];
+      const int lo = sg.row_start[q] > 0 ? sg.row_start[q] : 0, hi = sg.row_start[q + 1] < sg.M ? sg.row_start[q + 1] : sg.M;
+      if (lo >= hi) continue;
+      const int last = (hi - 1) / rows_per_run;
+#pragma unroll 4
+      for (int run = lo / rows_per_run; run <= last; ++run)
+        v += reinterpret_cast<const f32x4*>(o.part)[part_at<RT>(o, run + q, pb, rc, chunks) + tile * 64 + lane];
+    }
+  }
+  outer_store<T, RT>(o, v, tile, lane, a, pb, 64 * rc, rank);
+}
+
+// the same without partial sums, for so many requests that their slots would not fit: a workgroup sums all rows of an adapter
+template <typename T, int RT>
+__global__ __launch_bounds__(256) void k_outer_direct(Outer oa, Outer ob, Segs sg, KeepArgs ka, int rank) {
+  __shared__ ReqList list;
+  __shared__ f32x4 red[4][8][64];
+  const Outer& o = blockIdx.z == 0 ? oa : ob;
+  const int chunks = (rank + 63) / 64, a = blockIdx.y, pb = blockIdx.x / chunks, ib = 64 * (blockIdx.x % chunks);
+  if (pb >= o.blocks) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15;
+  const KeepKey key = keep_key(ka);
+  f32x4 acc[8][RT];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int i = 0; i < RT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int base = 0; base < sg.S; base += 256) {
+    list_requests(sg, a, base, &list);
+    for (int e = 0; e < list.n; ++e) {
+      const int q = list.q[e];
+      const int lo = sg.row_start[q] > 0 ? sg.row_start[q] : 0, hi = sg.row_start[q + 1] < sg.M ? sg.row_start[q + 1] : sg.M;
+      const T* X = static_cast<const T*>(o.X);
+      const int p = pb * OU_COLS + 8 * l16;
+      outer_rows<T, RT>(acc, X, o.ldx, o.P, o.t, rank, ib, p, lo, hi, w, lane, o.drop != 0, ka, key);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[w][j][lane] = acc[j][i];
+    __syncthreads();
+    for (int j = w; j < 8; j += 4)
+      outer_store<T, RT>(o, (red[0][j][lane] + red[1][j][lane]) + (red[2][j][lane] + red[3][j][lane]), j * RT + i, lane, a, pb, ib, rank);
+    __syncthreads();
+  }
+}
+
+// ---- transposes for the backward pass: out[z][c][r] = in[z][r][c] (rows x cols), out rows padded with zeros to ldo
+template <typename T>
+__global__ __launch_bounds__(256) void k_turn(const T* __restrict__ in, long long ldi, long long si, int rows, int cols,
+                                              T* __restrict__ out, long long ldo, long long so) {
+  __shared__ T tile[64][66];
+  const T* i = in + blockIdx.z * si;
+  T* o = out + blockIdx.z * so;
+  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  for (int j = ty; j < 64; j += 4)
+    tile[j][tx] = r0 + j < rows && c0 + tx < cols ? i[(r0 + j) * ldi + c0 + tx] : (T)0.f;
+  __syncthreads();
+  for (int j = ty; j < 64; j += 4)
+    if (c0 + j < cols && r0 + tx < ldo) o[(c0 + j) * ldo + r0 + tx] = tile[tx][j];
+}
+
+// ---- host side
+
+size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
+size_t type_size(int type) { return type == HM_TYPE_F32 ? 4 : 2; }
+
+struct Plan {
+  int rt, chunks, rows_per_run, runs, direct;
+  long long npad;
+  size_t wt, bt, u, pa, pb, total;       // offsets into the workspace
+};
+
+constexpr size_t MAX_PART = size_t(512) << 20;
+
+Plan make_plan(const hm_adapter_args& g) {
+  Plan p;
+  p.rt = g.rank <= 16 ? 1 : g.rank <= 32 ? 2 : 4;
+  p.chunks = (g.rank + 63) / 64;
+  const int ba = (g.k + OU_COLS - 1) / OU_COLS, bb = (g.n + OU_COLS - 1) / OU_COLS, blocks = ba > bb ? ba : bb;
+  // about 1024 workgroups (four a CU), runs of at least 64 rows
+  long long runs = (1024 + blocks - 1) / blocks, most = (g.rows + 63) / 64;
+  runs = runs < most ? runs : most;
+  if (runs < 1) runs = 1;
+  long long per = (g.rows + runs - 1) / runs;
+  per = (per + 15) & ~15ll;
+  if (per < 16) per = 16;
+  p.rows_per_run = (int)per;
+  p.runs = (int)((g.rows + per - 1) / per);
+  p.npad = (g.n + 7) & ~7ll;
+  const size_t slot = (size_t)p.chunks * 8 * p.rt * 64 * sizeof(f32x4), slots = (size_t)p.runs + g.segments;
+  p.direct = slots * slot * (ba + bb) > MAX_PART;
+  size_t at = 0;
+  p.wt = at; at = up256(at + (size_t)g.k * p.npad * type_size(g.type));
+  p.bt = at; at = up256(at + (size_t)g.adapters * g.rank * p.npad * type_size(g.type));
+  p.u = at;  at = up256(at + (size_t)g.rows * g.rank * sizeof(float));
+  p.pa = at; at = up256(at + (p.direct ? 0 : slots * slot * ba));
+  p.pb = at; at = up256(at + (p.direct ? 0 : slots * slot * bb));
+  p.total = at;
+  return p;
+}
+
+int check_args(const char* name, const hm_adapter_args* g, KeepArgs* ka) {
+  if (g == nullptr) { hm_set_error("%s: null argument", name); return -1; }
+  if (g->type < HM_TYPE_F32 || g->type > HM_TYPE_BF16) { hm_set_error("%s: unknown element type %d", name, g->type); return -1; }
+  if (g->rows < 0 || g->rows > HM_ADAPTER_MAX_ROWS) {
+    hm_set_error("%s: %lld rows, at most %d are taken", name, g->rows, HM_ADAPTER_MAX_ROWS); return -1; }
+  if (g->k < 1 || g->n < 1 || g->k > HM_ADAPTER_MAX_WIDTH || g->n > HM_ADAPTER_MAX_WIDTH) {
+    hm_set_error("%s: k = %d and n = %d must be in 1 .. %d", name, g->k, g->n, HM_ADAPTER_MAX_WIDTH); return -1; }
+  if (g->rank < 1 || g->rank > HM_ADAPTER_MAX_RANK) {
+    hm_set_error("%s: rank %d must be in 1 .. %d", name, g->rank, HM_ADAPTER_MAX_RANK); return -1; }
+  if (g->adapters < 0 || g->segments < 0 || g->adapters > HM_ADAPTER_MAX_COUNT || g->segments > HM_ADAPTER_MAX_ROWS) {
+    hm_set_error("%s: %d adapters (0 .. %d) and %d requests (0 .. %d) asked for", name, g->adapters, HM_ADAPTER_MAX_COUNT, g->segments,
+                 HM_ADAPTER_MAX_ROWS); return -1; }
+  if (!keep_args(ka, g->p, g->seed, g->d_seed, g->tag, g->row0)) {
+    hm_set_error("%s: p must be in [0, 1], got %g", name, g->p); return -1; }
+  if (g->rows > 0 && (g->d_x == nullptr || g->d_w == nullptr)) { hm_set_error("%s: null argument", name); return -1; }
+  if (g->adapters > 0 && g->segments > 0 &&
+      (g->d_a == nullptr || g->d_b == nullptr || g->d_row_start == nullptr || g->d_adapter == nullptr)) {
+    hm_set_error("%s: null argument", name); return -1; }
+  if ((g->rows > 1 && g->ld_x < g->k) || (g->n > 1 && g->ld_w < g->k)) {
+    hm_set_error("%s: a row stride is less than k = %d", name, g->k); return -1; }
+  return 0;
+}
+
+Segs segs_of(const hm_adapter_args& g) {
+  return {g.d_row_start, g.d_adapter, g.d_scale, g.adapters > 0 ? g.segments : 0, g.adapters, (int)g.rows};
+}
+
+// requests of fewer than eight rows on average: a wave per row.  A matrix product of the tiled kernel would be filled to less than
+// a quarter, once for each request in its 32 rows.
+bool few_rows_each(const hm_adapter_args& g) { return g.rows < 8ll * g.segments; }
+
+template <typename T>
+int shrink(const hm_adapter_args& g, const T* X, long long ldx, int K, const T* R, long long ldr, long long stride_a, bool drop,
+           const KeepArgs& ka, float* t, hipStream_t st) {
+  const Segs sg = segs_of(g);
+  const float f = drop ? ka.up : 1.f;
+  if (few_rows_each(g)) {
+    const long long waves = g.rows * ((g.rank + SR_RANKS - 1) / SR_RANKS);
+    const dim3 grid((unsigned)((waves + 3) / 4));
+    if (drop) hipLaunchKernelGGL((k_shrink_rows<T, true>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t);
+    else hipLaunchKernelGGL((k_shrink_rows<T, false>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t);
+  } else {
+    const dim3 grid((unsigned)((g.rows + SH_ROWS - 1) / SH_ROWS), (g.rank + SH_RANKS - 1) / SH_RANKS);
+#define HM_GO(RT, D) hipLaunchKernelGGL((k_shrink<T, RT, D>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t)
+    if (g.rank <= 16) { if (drop) HM_GO(1, true); else HM_GO(1, false); }
+    else if (g.rank <= 32) { if (drop) HM_GO(2, true); else HM_GO(2, false); }
+    else { if (drop) HM_GO(4, true); else HM_GO(4, false); }
+#undef HM_GO
+  }
+  HM_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+template <typename T>
+int project(const hm_adapter_args& g, const T* X, long long ldx, int Kk, const T* W, long long ldw, int Nn, const T* bias,
+            const LowRank& lr, bool drop, const KeepArgs& ka, T* out, long long ldo, hipStream_t st) {
+  const Segs sg = segs_of(g);
+  const long long tm = (g.rows + 127) / 128, tn = (Nn + 127) / 128;
+  const dim3 grid((unsigned)(tm * tn));
+  if (drop) hipLaunchKernelGGL((k_project<T, 128, 128, 2, 2, true>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, (int)tn);
+  else hipLaunchKernelGGL((k_project<T, 128, 128, 2, 2, false>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, (int)tn);
+  HM_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+template <typename T> int forward(const hm_adapter_args& g, const KeepArgs& ka, void* d_y, long long ld_y, float* d_t, hipStream_t st) {
+  const T *X = static_cast<const T*>(g.d_x), *W = static_cast<const T*>(g.d_w), *A = static_cast<const T*>(g.d_a);
+  const T* bias = static_cast<const T*>(g.d_bias);
+  T* y = static_cast<T*>(d_y);
+  const bool any = g.adapters > 0 && g.segments > 0;
+  if (any) {
+    const int rc = shrink<T>(g, X, g.ld_x, g.k, A, g.k, (long long)g.rank * g.k, ka.threshold != 0, ka, d_t, st);
+    if (rc) return rc;
+  }
+  const LowRank lr = {any ? d_t : nullptr, g.d_b, (long long)g.n * g.rank, g.rank, 1, g.rank};
+  if (g.rows <= FEW_ROWS) {
+    const dim3 grid((g.n + 15) / 16);
+    const Segs sg = segs_of(g);
+#define HM_GO(MT) hipLaunchKernelGGL((k_project_few<T, MT>), grid, dim3(64 * FEW_WAVES), 0, st, X, g.ld_x, g.k, W, g.ld_w, g.n, bias, lr, sg, y, ld_y)
+    if (g.rows <= 16) HM_GO(1);
+    else if (g.rows <= 32) HM_GO(2);
+    else HM_GO(4);
+#undef HM_GO
+    HM_CHECK_HIP(hipGetLastError());
+    return 0;
+  }
+  return project<T>(g, X, g.ld_x, g.k, W, g.ld_w, g.n, bias, lr, false, ka, y, ld_y, st);
+}
+
+template <typename T>
+int turn(const T* in, long long ldi, long long si, int rows, int cols, T* out, long long ldo, long long so, int count, hipStream_t st) {
+  hipLaunchKernelGGL((k_turn<T>), dim3((cols + 63) / 64, (unsigned)((ldo + 63) / 64), count), dim3(256), 0, st, in, ldi, si, rows, cols, out, ldo, so);
+  HM_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+template <typename T>
+int backward(const hm_adapter_args& g, const KeepArgs& ka, const void* d_dy, long long ld_dy, const float* d_t, void* d_dx,
+             long long ld_dx, void* d_da, void* d_db, char* ws, hipStream_t st) {
+  const Plan p = make_plan(g);
+  const T *X = static_cast<const T*>(g.d_x), *W = static_cast<const T*>(g.d_w), *dy = static_cast<const T*>(d_dy);
+  T *wt = reinterpret_cast<T*>(ws + p.wt), *bt = reinterpret_cast<T*>(ws + p.bt);
+  float* u = reinterpret_cast<float*>(ws + p.u);
+  const bool any = g.adapters > 0 && g.segments > 0 && g.rows > 0;
+  int rc;
+  if (any && (d_dx != nullptr || d_da != nullptr)) {
+    if ((rc = turn<T>(static_cast<const T*>(g.d_b), g.rank, (long long)g.n * g.rank, g.n, g.rank, bt, p.npad, g.rank * p.npad, g.adapters, st))) return rc;
+    if ((rc = shrink<T>(g, dy, ld_dy, g.n, bt, p.npad, g.rank * p.npad, false, ka, u, st))) return rc;
+    // u carries s_a; the factor of the dropout joins where the mask does
+  }
+  if (d_dx != nullptr && g.rows > 0) {
+    if ((rc = turn<T>(W, g.ld_w, 0, g.n, g.k, wt, p.npad, 0, 1, st))) return rc;
+    const LowRank lr = {any ? u : nullptr, g.d_a, (long long)g.rank * g.k, 1, g.k, g.rank};
+    if ((rc = project<T>(g, dy, ld_dy, g.n, wt, p.npad, g.k, nullptr, lr, ka.threshold != 0, ka, static_cast<T*>(d_dx), ld_dx, st))) return rc;
+  }
+  if (g.adapters > 0 && (d_da != nullptr || d_db != nullptr)) {
+    const Segs sg = segs_of(g);
+    Outer oa = {X, g.ld_x, d_da != nullptr ? g.k : 0, u, d_da, (long long)g.rank * g.k, 1, g.k, reinterpret_cast<float*>(ws + p.pa),
+                d_da != nullptr ? (g.k + OU_COLS - 1) / OU_COLS : 0, ka.threshold != 0, ka.up};
+    Outer ob = {dy, ld_dy, d_db != nullptr ? g.n : 0, d_t, d_db, (long long)g.n * g.rank, g.rank, 1, reinterpret_cast<float*>(ws + p.pb),
+                d_db != nullptr ? (g.n + OU_COLS - 1) / OU_COLS : 0, 0, 1.f};
+    const int blocks = oa.blocks > ob.blocks ? oa.blocks : ob.blocks;
+#define HM_GO(RT)                                                                                                                    \
+    if (p.direct) {                                                                                                                  \
+      hipLaunchKernelGGL((k_outer_direct<T, RT>), dim3(blocks * p.chunks, g.adapters, 2), dim3(256), 0, st, oa, ob, sg, ka, g.rank); \
+    } else {                                                                                                                         \
+      if (any) hipLaunchKernelGGL((k_outer<T, RT>), dim3(blocks, p.runs, 2), dim3(256), 0, st, oa, ob, sg, ka, g.rank, p.rows_per_run); \
+      hipLaunchKernelGGL((k_outer_sum<T, RT>), dim3(blocks * p.chunks * 2 * RT, g.adapters, 2), dim3(256), 0, st, oa, ob, sg, g.rank, p.rows_per_run); \
+    }
+    if (p.rt == 1) { HM_GO(1) } else if (p.rt == 2) { HM_GO(2) } else { HM_GO(4) }
+#undef HM_GO
+    HM_CHECK_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int hm_adapter_linear(const hm_adapter_args* g, void* d_y, long long ld_y, float* d_t, void* stream) {
+  KeepArgs ka;
+  const int rc = check_args("hm_adapter_linear", g, &ka);
+  if (rc) return rc;
+  if (g->rows == 0) return 0;
+  if (d_y == nullptr || (d_t == nullptr && g->adapters > 0 && g->segments > 0)) { hm_set_error("hm_adapter_linear: null argument"); return -1; }
+  if (g->rows > 1 && ld_y < g->n) { hm_set_error("hm_adapter_linear: row stride %lld of the output is less than n = %d", ld_y, g->n); return -1; }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (g->type == HM_TYPE_F32) return forward<float>(*g, ka, d_y, ld_y, d_t, st);
+  if (g->type == HM_TYPE_F16) return forward<f16>(*g, ka, d_y, ld_y, d_t, st);
+  return forward<bf16>(*g, ka, d_y, ld_y, d_t, st);
+}
+
+extern "C" long long hm_adapter_linear_backward_bytes(const hm_adapter_args* g) {
+  KeepArgs ka;
+  hm_adapter_args h;
+  if (g != nullptr) {                                  // sizes alone count here
+    h = *g;
+    h.rows = 0; h.segments = 0; h.ld_x = g->k; h.ld_w = g->k;
+    if (g->rows < 0 || g->rows > HM_ADAPTER_MAX_ROWS || g->segments < 0 || g->segments > HM_ADAPTER_MAX_ROWS) h.rows = -1;
+  }
+  if (check_args("hm_adapter_linear_backward_bytes", g != nullptr ? &h : nullptr, &ka)) return -1;
+  return (long long)make_plan(*g).total;
+}
+
+extern "C" int hm_adapter_linear_backward(const hm_adapter_args* g, const void* d_dy, long long ld_dy, const float* d_t, void* d_dx,
+                                          long long ld_dx, void* d_da, void* d_db, void* d_ws, long long ws_bytes, void* stream) {
+  KeepArgs ka;
+  const int rc = check_args("hm_adapter_linear_backward", g, &ka);
+  if (rc) return rc;
+  const bool any = g->rows > 0 && g->adapters > 0 && g->segments > 0;
+  if ((g->rows > 0 && d_dy == nullptr) || (any && d_db != nullptr && d_t == nullptr)) {
+    hm_set_error("hm_adapter_linear_backward: null argument"); return -1; }
+  if (g->rows > 1 && (ld_dy < g->n || (d_dx != nullptr && ld_dx < g->k))) {
+    hm_set_error("hm_adapter_linear_backward: a row stride is less than the columns"); return -1; }
+  const Plan p = make_plan(*g);
+  if (d_ws == nullptr || ws_bytes < (long long)p.total) {
+    hm_set_error("hm_adapter_linear_backward: workspace of %lld bytes, %lld are needed", d_ws == nullptr ? 0ll : ws_bytes, (long long)p.total); return -1; }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(d_ws);
+  if (g->type == HM_TYPE_F32) return backward<float>(*g, ka, d_dy, ld_dy, d_t, d_dx, ld_dx, d_da, d_db, ws, st);
+  if (g->type == HM_TYPE_F16) return backward<f16>(*g, ka, d_dy, ld_dy, d_t, d_dx, ld_dx, d_da, d_db, ws, st);
+  return backward<bf16>(*g, ka, d_dy, ld_dy, d_t, d_dx, ld_dx, d_da, d_db, ws, st);
+}

@@ -335,6 +335,73 @@ int hm_prep_dbscan(const double* d_pts, const int* d_n_pts, int n_stride, int B,
 int hm_prep_box_select(const double* d_pts, int n, const double* d_boxes, int B, int gather, int* d_counts,
                        const long long* d_offsets, int* d_idx, void* stream);
 
+/* ---- training and adapting decoders: the operators beside the projections of a DeepSDF decoder in a training step (the
+ * reference trains with dropout 0.2 behind every hidden layer, deepsdf/networks/deep_sdf_decoder.py:96-104).  Rows are points (or
+ * tokens), row-major with a row stride in elements; element types HM_TYPE_*; sums are held in 32 bits.  Pure enqueues: nothing is
+ * allocated and nothing waits, so the calls may be captured into a graph. */
+#define HM_TYPE_F32 0
+#define HM_TYPE_F16 1
+#define HM_TYPE_BF16 2
+
+/* Dropout whose mask is never stored: y = keep ? act(x) / (1 - p) : 0, act = ReLU when `relu`, else the identity.  keep comes
+ * from the counter-based generator Philox4x32-10: key = (low, high 32 bits of the seed), counter = (column / 8, row low, row high,
+ * tag), its four words being eight 16-bit draws, low half first, for the eight columns of a block; a value is kept where its draw
+ * is >= round(65536 p), so p is taken to the nearest 1 / 65536 (p < 1 keeps something, p = 1 nothing).  A decision depends on
+ * (seed, tag, row, column) alone.
+ *   seed    the 64-bit seed; d_seed (or NULL): a device word added to it, read when the kernel runs -- what a replayed graph changes
+ *   tag     tells streams of one seed apart (a layer's number);  row0: number of the first row (a shard, a chunk of a batch)
+ * hm_dropout_backward: dx from dy.  relu != 0: from d_y, the forward's OUTPUT (0 where nothing passed; nothing is drawn);
+ * relu == 0: d_y is not read, the draws are made again from the same seed, tag, row0 and p. */
+int hm_dropout(const void* d_x, long long ld_x, void* d_y, long long ld_y, long long rows, int cols, int type, int relu, double p,
+               unsigned long long seed, const unsigned long long* d_seed, unsigned tag, unsigned long long row0, void* stream);
+int hm_dropout_backward(const void* d_dy, long long ld_dy, const void* d_y, long long ld_y, void* d_dx, long long ld_dx,
+                        long long rows, int cols, int type, int relu, double p, unsigned long long seed,
+                        const unsigned long long* d_seed, unsigned tag, unsigned long long row0, void* stream);
+
+/* Low-rank adapters of many requests at once beside a shared, frozen projection:
+ *   y[m] = x[m] W^T + bias + scale[a] drop(x[m]) A[a]^T B[a]^T,      a = adapter[q] of the request q that holds row m.
+ * Request q holds the rows row_start[q] .. row_start[q + 1] - 1 (ascending; empty requests are fine).  adapter[q] outside
+ * 0 .. adapters - 1, and rows of no request, leave the bare projection.  drop is hm_dropout's (p = 0: none) with the same
+ * seed / d_seed / tag / row0.  row_start and adapter are device arrays that the host never reads: a row_start that does not
+ * ascend gives unspecified values for the rows concerned, nothing else.
+ * A row's result depends on its own row and adapter alone (not on the batch around it, bit for bit as long as the same kernels
+ * run; an infinity or NaN in another request or adapter does not reach it). */
+#define HM_ADAPTER_MAX_ROWS 16777216
+#define HM_ADAPTER_MAX_WIDTH 65536
+#define HM_ADAPTER_MAX_RANK 256
+#define HM_ADAPTER_MAX_COUNT 65535
+typedef struct hm_adapter_args {
+  int type;                /* HM_TYPE_* of x, w, bias, a, b and of the results                       */
+  int k, n, rank;          /* x (rows, k) -> y (rows, n)                                              */
+  int adapters, segments;  /* adapters in a / b; requests                                             */
+  unsigned tag;
+  long long rows;
+  const void* d_x;         /* [rows][k], row stride ld_x                                              */
+  long long ld_x;
+  const void* d_w;         /* [n][k], row stride ld_w                                                 */
+  long long ld_w;
+  const void* d_bias;      /* [n] or NULL                                                             */
+  const void* d_a;         /* [adapters][rank][k]                                                     */
+  const void* d_b;         /* [adapters][n][rank]                                                     */
+  const float* d_scale;    /* [adapters] or NULL: 1                                                   */
+  const int* d_row_start;  /* [segments + 1]                                                          */
+  const int* d_adapter;    /* [segments]                                                              */
+  double p;
+  unsigned long long seed;
+  const unsigned long long* d_seed;
+  unsigned long long row0;
+} hm_adapter_args;
+
+/* d_t [rows][rank] floats: scale[a] drop(x) A[a]^T / (1 - p) of the rows that have an adapter; scratch, and what the backward pass
+ * reads.  Not used (may be NULL) when adapters or segments is 0. */
+int hm_adapter_linear(const hm_adapter_args* args, void* d_y, long long ld_y, float* d_t, void* stream);
+/* Gradients, each where its pointer is not NULL: d_dx [rows][k], d_da like a, d_db like b (zeros for an adapter without rows).
+ * The projection and the scales get none.  d_ws: workspace of at least hm_adapter_linear_backward_bytes(args) bytes (-1 on an
+ * error), 256-byte aligned, used by this call alone while it runs; sums run in a fixed order (no atomics). */
+long long hm_adapter_linear_backward_bytes(const hm_adapter_args* args);
+int hm_adapter_linear_backward(const hm_adapter_args* args, const void* d_dy, long long ld_dy, const float* d_t, void* d_dx,
+                               long long ld_dx, void* d_da, void* d_db, void* d_ws, long long ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,323 @@
+"""Low-rank adapters of many requests beside a shared projection (hm_adapter_linear) against a 64-bit restatement.
+
+Tolerance of a sum of n products held in 32 bits, in whatever order: (n + 8) steps of 2^-23 of the sum of the absolute values
+(each addition off by at most one step of a partial sum no larger than that), and half a step of the type for the one rounding
+at the end.  What stands between the two products of the adapters is a sum of its own (n counts both) and is split into a high
+and a low 16-bit part: off by 2^-16 of itself (bf16: half a step of the low part, 2^-8 of 2^-8), of its share of the sum."""
+import numpy as np
+import pytest
+import torch
+
+import adapter_oracle as AO
+from hortimapping_amd import ops
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def normal(shape, dtype, seed, std=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+class Case:
+    def __init__(self, rows, k, n, r, lengths, which, na, dtype, seed=0, bias=True, scale=True, start=0):
+        self.rows, self.k, self.n, self.r, self.na, self.dtype = rows, k, n, r, na, dtype
+        self.start = [start]
+        for v in lengths:
+            self.start.append(self.start[-1] + v)
+        self.which = list(which)
+        assert self.start[-1] <= rows and len(self.which) == len(lengths)
+        self.x = normal((rows, k), dtype, seed).requires_grad_()
+        self.W = normal((n, k), dtype, seed + 1, k ** -0.5)
+        self.A = normal((na, r, k), dtype, seed + 2, k ** -0.5).requires_grad_()
+        self.B = normal((na, n, r), dtype, seed + 3, 0.5 * r ** -0.5).requires_grad_()
+        self.b = normal((n,), dtype, seed + 4) if bias else None
+        self.scale = normal((na,), torch.float32, seed + 5).abs() + 0.3 if scale else None
+        self.dy = normal((rows, n), dtype, seed + 6, 0.1)
+        self.row_start = torch.tensor(self.start, dtype=torch.int32, device="cuda")
+        self.adapter = torch.tensor(self.which, dtype=torch.int32, device="cuda")
+
+    def call(self, **kw):
+        return ops.adapter_linear(self.x, self.W, self.A, self.B, self.row_start, self.adapter, bias=self.b, scale=self.scale, **kw)
+
+    def check(self, backward=True, p=0.0, seed=0, tag=0):
+        y = self.call(p=p, seed=seed, tag=tag)
+        got = [y]
+        if backward:
+            got += list(torch.autograd.grad(y, (self.x, self.A, self.B), self.dy))
+        keep, up = AO.keep_mask(self.rows, self.k, p, seed, tag) if p > 0 else (None, 1.0)
+        ra = AO.segment_of_rows(self.start, self.which, self.rows, self.na)
+        ref = [AO.adapter_linear(self.x, self.W, self.b, self.A, self.B, self.scale, ra, keep, up, self.dy if backward else None, m)
+               for m in (False, True)]
+        want, size = ref if backward else ([ref[0]], [ref[1]])
+        most = max([0] + [int((ra == i).sum()) for i in range(self.na)])
+        split = 0.0 if self.dtype == torch.float32 else 2.0 ** -16
+        f = torch.finfo(self.dtype)
+        count = (self.k + 2 * self.r, self.n + 2 * self.r, most + self.n, most + self.k)
+        for name, g, w, s, c in zip(("y", "dx", "dA", "dB"), got, want, size, count):
+            assert g.dtype == self.dtype and tuple(g.shape) == tuple(w.shape), name
+            err = (g.detach().double().cpu() - w).abs()
+            tol = ((c + 8) * 2.0 ** -23 + split) * s + f.eps / 2 * w.abs() + f.smallest_normal * f.eps
+            assert bool((err <= tol).all()), (name, float((err / tol).max()), float(err.max()))
+        return got
+
+
+# rows, K, N, rank, lengths, adapters used, adapters
+LAYOUTS = {
+    "one row": (1, 8, 8, 4, [1], [0], 1),
+    "one value": (1, 1, 1, 1, [1], [0], 1),
+    "single rows": (9, 512, 512, 8, [1] * 9, [3, 0, -1, 2, 2, 7, 1, 0, 3], 4),          # -1 and 7: no adapter
+    "single rows odd": (40, 259, 253, 13, [1] * 40, [i % 5 for i in range(40)], 5),
+    "few rows": (64, 70, 33, 5, [30, 0, 34], [1, 0, 0], 2),
+    "one more": (65, 64, 128, 16, [65], [0], 1),
+    "ragged": (300, 259, 130, 7, [5, 0, 100, 1, 64, 30], [2, 1, 0, -1, 2, 1], 3),       # rows behind the last request
+    "short": (301, 130, 70, 33, [7] * 43, [i % 4 for i in range(43)], 4),
+    "tile crossing": (520, 64, 256, 64, [127, 2, 130, 261], [0, 1, 2, 1], 3),
+    "big rank": (150, 96, 140, 70, [70, 80], [1, 0], 2),
+    "bigger rank": (140, 40, 48, 256, [140], [0], 1),
+    "no adapter": (130, 64, 64, 8, [100], [-1], 2),
+    "unused adapter": (200, 128, 96, 16, [200], [1], 3),
+    "wide": (257, 1031, 515, 16, [129, 128], [0, 1], 2),
+}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", sorted(LAYOUTS))
+def test_forward_and_backward(name, dtype):
+    c = Case(*LAYOUTS[name], dtype)
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["single rows odd", "few rows", "ragged", "short", "tile crossing", "big rank", "wide"])
+def test_with_dropout_on_the_input(name, dtype):
+    c = Case(*LAYOUTS[name], dtype, seed=40)
+    c.check(p=0.3, seed=(1 << 45) + 17, tag=2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_without_bias_scale_or_first_rows(dtype):
+    Case(150, 72, 65, 6, [20, 90], [1, 0], 2, dtype, bias=False, scale=False, start=11).check()
+    Case(20, 72, 65, 6, [5, 3], [1, 0], 2, dtype, bias=False, scale=False, start=11).check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_sizes_of_the_decoder(dtype):
+    """First layer, the layer before the skip connection, a hidden layer: a few thousand points of eight instances."""
+    for k, n, r, p in ((259, 512, 8, 0.2), (512, 253, 16, 0.0), (512, 512, 4, 0.2)):
+        Case(5000, k, n, r, [1000, 300, 0, 700, 1024, 512, 900, 500], [0, 1, 2, 3, 0, -1, 2, 1], 4, dtype, seed=k).check(p=p, seed=5)
+
+
+def test_no_requests_and_no_rows():
+    c = Case(70, 32, 48, 4, [], [], 2, torch.float32)
+    y, dx, dA, dB = c.check()
+    assert not dA.any() and not dB.any()
+    x = torch.zeros(0, 32, device="cuda", requires_grad=True)
+    y = ops.adapter_linear(x, c.W, c.A, c.B, c.row_start, c.adapter)
+    assert y.shape == (0, 48)
+    dx, dA = torch.autograd.grad(y.sum(), (x, c.A))
+    assert dx.shape == (0, 32) and dA.shape == c.A.shape and not dA.any()
+    none = [t.detach()[:0] for t in (c.A, c.B)]
+    y = ops.adapter_linear(c.x.detach(), c.W, *none, c.row_start, c.adapter, bias=c.b)
+    want = c.x.detach().double() @ c.W.double().t() + c.b.double()
+    assert float((y.double() - want).abs().max()) < 40 * 2.0 ** -23 * 40
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,lengths", [(12, [1] * 12), (300, [100, 60, 140])])
+def test_the_mask_is_that_of_dropout(dtype, rows, lengths):
+    """adapter_linear(p) equals the bare projection of x plus the adapters on ops.dropout(x): with weights of zero and exact
+    inputs (powers of two) bit for bit."""
+    which = [i % 2 for i in range(len(lengths))]
+    c = Case(rows, 64, 96, 4, lengths, which, 2, dtype)
+    x = torch.sign(c.x.detach())
+    A = torch.sign(c.A.detach()) * 0.25
+    B = torch.sign(c.B.detach())
+    zero = torch.zeros_like(c.W)
+    got = ops.adapter_linear(x, zero, A, B, c.row_start, c.adapter, p=0.5, seed=77, tag=4)
+    want = ops.adapter_linear(ops.dropout(x, 0.5, 77, tag=4), zero, A, B, c.row_start, c.adapter)
+    assert torch.equal(got, want) and bool(got.any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides(dtype):
+    """Rows of a wider buffer at odd places, a weight that is a slice, leading dimensions, gradients of any strides."""
+    c = Case(150, 67, 51, 5, [50, 100], [1, 0], 2, dtype)
+    c.check()
+    wide = torch.zeros(150, 97, dtype=dtype, device="cuda")
+    wide[:, 3:70] = c.x.detach()
+    ww = torch.zeros(51, 99, dtype=dtype, device="cuda")
+    ww[:, 1:68] = c.W
+    x = wide[:, 3:70].view(3, 50, 67).requires_grad_()
+    y = ops.adapter_linear(x, ww[:, 1:68], c.A, c.B, c.row_start, c.adapter, bias=c.b, scale=c.scale)
+    ref = c.call()
+    assert y.shape == (3, 50, 51) and torch.equal(y.view(150, 51), ref)
+    dy = c.dy[:1, :1].expand(150, 51)
+    a = torch.autograd.grad(y, (x, c.A, c.B), dy.reshape(3, 50, 51), retain_graph=True)
+    b = torch.autograd.grad(ref, (c.x, c.A, c.B), dy)
+    assert torch.equal(a[0].view(150, 67), b[0]) and torch.equal(a[1], b[1]) and torch.equal(a[2], b[2])
+    t = normal((51, 150), dtype, 9).t()
+    ref = c.call()
+    assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(ref, (c.x, c.A, c.B), t, retain_graph=True),
+                                                 torch.autograd.grad(ref, (c.x, c.A, c.B), t.contiguous())))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,lengths", [(16, [4, 4, 4, 4]), (40, [1] * 40), (400, [130, 20, 130, 120])])
+def test_an_infinity_stays_in_its_request(dtype, rows, lengths):
+    """A broken adapter and a broken row reach their own rows and nothing else."""
+    which = [i % 3 for i in range(len(lengths))]
+    c = Case(rows, 64, 96, 8, lengths, which, 3, dtype)
+    clean = [v.clone() for v in c.check()]
+    ra = torch.from_numpy(AO.segment_of_rows(c.start, c.which, rows, 3)).cuda()
+    with torch.no_grad():
+        c.A[1].fill_(float("nan"))
+        c.B[1].fill_(float("inf"))
+        c.x[0, 5] = float("inf")                       # request 0, adapter 0
+    y = c.call()
+    dx, dA, dB = torch.autograd.grad(y, (c.x, c.A, c.B), c.dy)
+    fine = (ra != 1)
+    fine[0] = False
+    assert torch.equal(y[fine], clean[0][fine])
+    assert bool((~torch.isfinite(y[ra == 1])).all())
+    other = ra != 1                                    # dx does not see x
+    assert torch.equal(dx[other], clean[1][other])
+    assert torch.equal(dA[2], clean[2][2]) and torch.equal(dB[2], clean[3][2])
+    assert bool(torch.isnan(dA[1]).any()) and bool((~torch.isfinite(dA[0][:, 5])).all())
+    assert torch.equal(dA[0][:, :5], clean[2][0][:, :5]) and torch.equal(dA[0][:, 6:], clean[2][0][:, 6:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_request_sees_the_batch_around_it(dtype):
+    """The rows of a request are the same bits whatever the other requests hold."""
+    a = Case(700, 128, 160, 16, [200, 300, 200], [0, 1, 2], 3, dtype)
+    y = a.call(p=0.25, seed=3).detach()
+    with torch.no_grad():
+        a.x[:200].mul_(2)
+        a.x[500:].zero_()
+    assert torch.equal(a.call(p=0.25, seed=3)[200:500], y[200:500])
+
+
+@pytest.mark.parametrize("rows,lengths,na", [(3000, [300] * 10, 3), (2000, [2] * 1000, 5)])
+def test_same_bits_every_time(rows, lengths, na):
+    c = Case(rows, 96, 130, 16, lengths, [i % na for i in range(len(lengths))], na, torch.bfloat16)
+    a, b = c.check(p=0.1, seed=9), c.check(p=0.1, seed=9)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_so_many_requests_that_partial_sums_would_not_fit():
+    """20000 requests of one row: sums over rows without slots."""
+    rows = 20000
+    c = Case(rows, 512, 140, 16, [1] * rows, [i % 7 - 1 for i in range(rows)], 6, torch.float32)
+    c.check()
+
+
+@pytest.mark.parametrize("start", [[0, 50, 30, 100], [0, 90, 20, 100], [-5, 40, 200, 100], [100, 60, 20, 0], [0, 2 ** 31 - 1, -2 ** 31, 7]])
+def test_row_starts_that_do_not_ascend_stay_in_bounds(start):
+    """Values of the rows concerned are unspecified; the call returns, and the next one is right."""
+    c = Case(100, 64, 64, 8, [40, 30, 30], [0, 1, 0], 2, torch.float32)
+    rs = torch.tensor(start, dtype=torch.int32, device="cuda")
+    for x in (c.x, c.x[:10].detach().requires_grad_()):
+        y = ops.adapter_linear(x, c.W, c.A, c.B, rs, c.adapter, bias=c.b, scale=c.scale)
+        torch.autograd.grad(y.sum(), (x, c.A, c.B))
+    torch.cuda.synchronize()
+    c.check()
+
+
+def test_gradient_against_differences():
+    """<gradient, direction> against a central difference of the outputs in 64 bits: the map is bilinear in (A, B) and linear in
+    x, so a difference in one of them is exact up to the rounding of the outputs."""
+    c = Case(90, 48, 40, 6, [30, 60], [1, 0], 2, torch.float32, seed=3)
+    y = c.call(p=0.2, seed=8)
+    grads = torch.autograd.grad(y, (c.x, c.A, c.B), c.dy)
+    for leaf, g in zip((c.x, c.A, c.B), grads):
+        d = torch.sign(normal(leaf.shape, torch.float32, 77))
+        h, keep = 2.0 ** -4, leaf.detach().clone()
+        with torch.no_grad():
+            leaf.copy_(keep + h * d)
+            up = c.call(p=0.2, seed=8).double()
+            leaf.copy_(keep - h * d)
+            down = c.call(p=0.2, seed=8).double()
+            leaf.copy_(keep)
+        diff = float((((up - down) / (2 * h)) * c.dy.double()).sum())
+        # 3600 outputs below 40, each off by (48 + 2 * 6 + 8) 2^-23 of it in either call, weighted with |dy|, over 2 h
+        tol = 2 * 68 * 2.0 ** -23 * 40 / (2 * h) * float(c.dy.double().abs().sum()) + 1e-5 * abs(diff)
+        assert abs(float((g.double() * d.double()).sum()) - diff) <= tol
+
+
+def test_graph_replays_with_other_requests_and_seeds():
+    c = Case(260, 64, 96, 8, [100, 60, 100], [0, 1, 2], 3, torch.bfloat16)
+    word = torch.zeros(1, dtype=torch.int64, device="cuda")
+
+    def step():
+        y = c.call(p=0.25, seed=word)
+        return [y] + list(torch.autograd.grad(y, (c.x, c.A, c.B), c.dy))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for seed, start, which in ((1, [0, 100, 160, 260], [0, 1, 2]), (2, [0, 7, 7, 200], [2, 0, -1]), (1 << 50, [3, 130, 131, 260], [1, 1, 0]),
+                               (1, [0, 100, 160, 260], [0, 1, 2])):
+        word.fill_(seed)
+        c.row_start.copy_(torch.tensor(start, dtype=torch.int32))
+        c.adapter.copy_(torch.tensor(which, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))        # eager work between the replays
+
+
+def test_two_streams_at_once():
+    cs = [Case(3000, 256, 256, 16, [1000, 500, 1500], [0, 1, 2], 3, torch.bfloat16, seed=i) for i in range(2)]
+
+    def step(c):
+        y = c.call()
+        return [y] + list(torch.autograd.grad(y, (c.x, c.A, c.B), c.dy))
+    want = [step(c) for c in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    got = []
+    for _ in range(3):
+        for c, s in zip(cs, streams):
+            with torch.cuda.stream(s):
+                got.append(step(c))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
+def test_gradients_asked_for_alone():
+    c = Case(300, 64, 96, 8, [100, 200], [0, 1], 2, torch.float32)
+    full = c.check()[1:]
+    for i in range(3):
+        leaves = [c.x, c.A, c.B]
+        for j, v in enumerate(leaves):
+            v.requires_grad_(j == i)
+        (g,) = torch.autograd.grad(c.call(), leaves[i], c.dy)
+        assert torch.equal(g, full[i])
+        for v in leaves:
+            v.requires_grad_(True)
+
+
+def test_refusals():
+    c = Case(70, 32, 48, 4, [30, 40], [0, 1], 2, torch.float32)
+    base = dict(x=c.x, weight=c.W, A=c.A, B=c.B, row_start=c.row_start, adapter=c.adapter, bias=c.b, scale=c.scale)
+    W = c.W.clone().requires_grad_()
+    bad = [dict(x=c.x.double()), dict(x=c.x[:, :31]), dict(x=c.x.half()), dict(x=c.x.detach().t().contiguous().t()),
+           dict(weight=c.W.t()), dict(weight=W), dict(weight=c.W.half()), dict(A=c.A[:1]), dict(A=c.A.transpose(0, 1)), dict(B=c.B[:, :, :2]),
+           dict(B=c.B.transpose(1, 2).contiguous().transpose(1, 2)), dict(bias=c.b[:3]), dict(bias=c.b.clone().requires_grad_()),
+           dict(scale=c.scale.double()), dict(scale=c.scale.clone().requires_grad_()), dict(scale=c.scale[:1]), dict(row_start=c.row_start.long()),
+           dict(row_start=c.row_start[:2]), dict(adapter=c.adapter.cpu()), dict(p=1.1), dict(p=float("nan")), dict(seed=-1), dict(seed=c.scale)]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            ops.adapter_linear(**{**base, **kw})
+    with torch.no_grad():                                                 # frozen or not does not matter without gradients
+        ops.adapter_linear(**{**base, "weight": W})
+    r = torch.zeros(2, 300, 32, device="cuda"), torch.zeros(2, 48, 300, device="cuda")
+    from hortimapping_amd._lib import HortiHipError
+    with pytest.raises(HortiHipError, match="rank 300"):
+        ops.adapter_linear(**{**base, "A": r[0], "B": r[1]})
