@@ -92,24 +92,31 @@ template <typename T> __device__ __forceinline__ Frag8<T> frag_load(const T* p, 
   }
   return f;
 }
+template <typename T> __device__ __forceinline__ Frag8<T> frag_load(const T* p) {
+  Frag8<T> f;
+  const Pack8<T> u = *reinterpret_cast<const Pack8<T>*>(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f.v[j] = u.v[j];
+  return f;
+}
 template <typename T> __device__ __forceinline__ void frag_keep(Frag8<T>& f, uint32_t keep) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) f.v[j] = (keep >> j) & 1 ? f.v[j] : (T)0.f;
 }
 
 // ---- t / u: 32 rows x up to 64 ranks per workgroup, the four waves share the reduction.  Bound by reading X once.
-constexpr int SH_ROWS = 32, SH_RANKS = 64;
+constexpr int SH_ROWS = 32, SH_RANKS = 64, SH_AHEAD = 4;
 
 template <typename T, int RT, bool DROP>
 __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ R, long long ldr,
                                                 long long stride_a, int rank, float factor, Segs sg, KeepArgs ka,
-                                                float* __restrict__ t) {
+                                                float* __restrict__ t, int ldt) {
   __shared__ f32x4 red[4][2 * RT][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
   const int r0 = blockIdx.x * SH_ROWS, ib = blockIdx.y * SH_RANKS;
   const int r1 = r0 + SH_ROWS < sg.M ? r0 + SH_ROWS : sg.M;
   const KeepKey key = keep_key(ka);
-  const int steps = (K + 31) >> 5;
+  const int full = K >> 5;
   int q = seg_find(sg, r0);
   for (q = q < 0 ? 0 : q; q < sg.S && sg.row_start[q] < r1; ++q) {
     const Span sp = seg_span(sg, q, r0, r1);
@@ -119,28 +126,55 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long lo
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int i = 0; i < RT; ++i) acc[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const T* Ra = R + (long long)sp.a * stride_a;
-    for (int s = w; s < steps; s += 4) {
-      const int k = 32 * s + 8 * g, n = K - k;
-      Frag8<T> x[2], a[RT];
+    // rows past the end and ranks past the rank are read as the last one: they touch their own results alone
+    const T *xp[2], *ap[RT];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const int row = r0 + 16 * m + l16;
-        x[m] = frag_load(X + row * ldx + k, row < sg.M ? n : 0);
-      }
+    for (int m = 0; m < 2; ++m) { const int row = r0 + 16 * m + l16; xp[m] = X + (row < sg.M ? row : sg.M - 1) * ldx + 8 * g; }
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        const int ri = ib + 16 * i + l16;
-        a[i] = frag_load(Ra + ri * ldr + k, ri < rank ? n : 0);
-      }
+    for (int i = 0; i < RT; ++i) {
+      const int ri = ib + 16 * i + l16;
+      ap[i] = R + (long long)sp.a * stride_a + (ri < rank ? ri : rank - 1) * ldr + 8 * g;
+    }
+    auto step = [&](const Frag8<T> (&x)[2], const Frag8<T> (&a)[RT], int s) {
+      Frag8<T> xk[2] = {x[0], x[1]};
       if (DROP) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) frag_keep(x[m], keep8(ka, key, (uint64_t)(r0 + 16 * m + l16), (uint32_t)(k >> 3)));
+        for (int m = 0; m < 2; ++m) frag_keep(xk[m], keep8(ka, key, (uint64_t)(r0 + 16 * m + l16), (uint32_t)(4 * s + g)));
       }
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int i = 0; i < RT; ++i) acc[m][i] = mma16(a[i], x[m], acc[m][i]);
+        for (int i = 0; i < RT; ++i) acc[m][i] = mma16(a[i], xk[m], acc[m][i]);
+    };
+    int s = w;
+    for (; s + 4 * (SH_AHEAD - 1) < full; s += 4 * SH_AHEAD) {     // the loads of four steps in flight
+      Frag8<T> x[SH_AHEAD][2], a[SH_AHEAD][RT];
+#pragma unroll
+      for (int u = 0; u < SH_AHEAD; ++u) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) x[u][m] = frag_load(xp[m] + 32 * (s + 4 * u));
+#pragma unroll
+        for (int i = 0; i < RT; ++i) a[u][i] = frag_load(ap[i] + 32 * (s + 4 * u));
+      }
+#pragma unroll
+      for (int u = 0; u < SH_AHEAD; ++u) step(x[u], a[u], s + 4 * u);
+    }
+    for (; s < full; s += 4) {
+      Frag8<T> x[2], a[RT];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) x[m] = frag_load(xp[m] + 32 * s);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) a[i] = frag_load(ap[i] + 32 * s);
+      step(x, a, s);
+    }
+    if (K > 32 * full && w == (full & 3)) {
+      const int n = K - 32 * full - 8 * g;
+      Frag8<T> x[2], a[RT];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) x[m] = frag_load(xp[m] + 32 * full, n);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) a[i] = frag_load(ap[i] + 32 * full, n);
+      step(x, a, full);
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -157,7 +191,7 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long lo
       if (row >= sp.lo && row < sp.hi) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (i0 + j < rank) t[(long long)row * rank + i0 + j] = v[j] * f;
+          if (i0 + j < ldt) t[(long long)row * ldt + i0 + j] = i0 + j < rank ? v[j] * f : 0.f;
       }
     }
     __syncthreads();
@@ -170,8 +204,8 @@ constexpr int SR_RANKS = 4;
 template <typename T, bool DROP>
 __global__ __launch_bounds__(256) void k_shrink_rows(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ R, long long ldr,
                                                      long long stride_a, int rank, float factor, Segs sg, KeepArgs ka,
-                                                     float* __restrict__ t) {
-  const int lane = threadIdx.x & 63, groups = (rank + SR_RANKS - 1) / SR_RANKS;
+                                                     float* __restrict__ t, int ldt) {
+  const int lane = threadIdx.x & 63, groups = ldt / SR_RANKS;
   const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int row = (int)(id / groups), i0 = (int)(id % groups) * SR_RANKS;
   if (row >= sg.M) return;
@@ -182,15 +216,31 @@ __global__ __launch_bounds__(256) void k_shrink_rows(const T* __restrict__ X, lo
   const KeepKey key = keep_key(ka);
   const T* Ra = R + (long long)sp.a * stride_a;
   float acc[SR_RANKS] = {};
-  for (int k = 8 * lane; k < K; k += 512) {
-    Frag8<T> x = frag_load(X + row * ldx + k, K - k);
+  const T *xr = X + row * ldx, *ar[SR_RANKS];
+#pragma unroll
+  for (int i = 0; i < SR_RANKS; ++i) ar[i] = Ra + (i0 + i < rank ? i0 + i : rank - 1) * ldr;
+  auto step = [&](Frag8<T> x, const Frag8<T> (&a)[SR_RANKS], int k) {
     if (DROP) frag_keep(x, keep8(ka, key, (uint64_t)row, (uint32_t)(k >> 3)));
 #pragma unroll
-    for (int i = 0; i < SR_RANKS; ++i) {
-      const Frag8<T> a = frag_load(Ra + (i0 + i) * ldr + k, i0 + i < rank ? K - k : 0);
+    for (int i = 0; i < SR_RANKS; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[i] = fmaf((float)x.v[j], (float)a.v[j], acc[i]);
-    }
+      for (int j = 0; j < 8; ++j) acc[i] = fmaf((float)x.v[j], (float)a[i].v[j], acc[i]);
+  };
+  int k = 8 * lane;
+#pragma unroll 2
+  for (; k + 8 <= K; k += 512) {
+    Frag8<T> a[SR_RANKS];
+    const Frag8<T> x = frag_load(xr + k);
+#pragma unroll
+    for (int i = 0; i < SR_RANKS; ++i) a[i] = frag_load(ar[i] + k);
+    step(x, a, k);
+  }
+  if (k < K) {
+    Frag8<T> a[SR_RANKS];
+    const Frag8<T> x = frag_load(xr + k, K - k);
+#pragma unroll
+    for (int i = 0; i < SR_RANKS; ++i) a[i] = frag_load(ar[i] + k, K - k);
+    step(x, a, k);
   }
   const float f = factor * (sg.scale != nullptr ? sg.scale[sp.a] : 1.f);
 #pragma unroll
@@ -198,14 +248,16 @@ __global__ __launch_bounds__(256) void k_shrink_rows(const T* __restrict__ X, lo
     float v = acc[i];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    if (lane == i && i0 + i < rank) t[(long long)row * rank + i0 + i] = v * f;
+    if (lane == i) t[(long long)row * ldt + i0 + i] = i0 + i < rank ? v * f : 0.f;
   }
 }
 
 // ---- the projection with the low-rank part: out (M, Nn) = X (M, Kk) W^T (+ bias) + t Bt_a^T, tiles of BM x BN in LDS, rows of
-// 128 bytes along the reduction, 16-byte chunks XOR-ed with the row (conflict-free 16-byte reads)
+// 128 bytes along the reduction, 16-byte chunks XOR-ed with the row (conflict-free 16-byte reads).  Two LDS buffers and one
+// barrier a step: the step after next is on its way to registers while a step is computed.
 template <typename T> struct Lines { static constexpr int V = 16 / sizeof(T), KB = 128 / sizeof(T); };
 template <typename T> struct alignas(16) Line { T v[16 / sizeof(T)]; };
+template <typename T> struct alignas(sizeof(T)) LooseLine { T v[16 / sizeof(T)]; };     // the same at the alignment of one value
 
 __device__ __forceinline__ f32x16 mma32(uint4 a, uint4 b, f32x16 c, f16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -220,26 +272,24 @@ __device__ __forceinline__ f32x16 mma32(uint4 a, uint4 b, f32x16 c, float) {
   return c;
 }
 
+template <typename T> __device__ __forceinline__ uint4 line_load(const T* p) {
+  return __builtin_bit_cast(uint4, *reinterpret_cast<const LooseLine<T>*>(p));
+}
+// the first n values of a line (n <= 0: none), zero behind them
 template <typename T> __device__ __forceinline__ uint4 line_load(const T* p, int n) {
   constexpr int V = Lines<T>::V;
-  struct alignas(sizeof(T)) P { T v[V]; };
+  if (n >= V) return line_load(p);
   Line<T> o;
-  if (n >= V) {
-    const P u = *reinterpret_cast<const P*>(p);
 #pragma unroll
-    for (int j = 0; j < V; ++j) o.v[j] = u.v[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) o.v[j] = j < n ? p[j] : (T)0.f;
-  }
+  for (int j = 0; j < V; ++j) o.v[j] = j < n ? p[j] : (T)0.f;
   return __builtin_bit_cast(uint4, o);
 }
 
 struct LowRank {
-  const float* t;          // [M][rank], or nullptr: no adapters at all
-  const void* b;           // element (adapter a, output n, i) at a * sa + n * sn + i * si
-  long long sa, sn, si;
-  int rank;
+  const float* t;          // [M][ldt], zeros behind the rank, or nullptr: no adapters at all
+  const void* b;           // element (adapter a, output n, i) at a * sa + n * sn + i
+  long long sa, sn;
+  int rank, ldt;           // ldt: the rank rounded up to 8
 };
 
 template <typename T, int BM, int BN, int WGM, int WGN, bool DROP>
@@ -248,7 +298,10 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
                                                             KeepArgs ka, T* __restrict__ out, long long ldo, int tiles_n) {
   constexpr int NT = 64 * WGM * WGN, MI = BM / WGM / 32, NI = BN / WGN / 32, V = Lines<T>::V, KB = Lines<T>::KB;
   constexpr int RX = BM * 8 / NT, RW = BN * 8 / NT;
-  __shared__ uint4 sx[2][BM * 8], sw[2][BN * 8];
+  __shared__ uint4 lds[2 * (BM + BN) * 8];
+  __shared__ float sb[BN];
+  uint4 (*sx)[BM * 8] = reinterpret_cast<uint4 (*)[BM * 8]>(lds);
+  uint4 (*sw)[BN * 8] = reinterpret_cast<uint4 (*)[BN * 8]>(lds + 2 * BM * 8);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w % WGM, wn = w / WGM, l32 = lane & 31, h = lane >> 5;
   // consecutive workgroups go to the eight XCDs in turn: give each XCD a contiguous run of tiles, so that the tiles that share
   // rows of X share an L2
@@ -256,6 +309,54 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
   const int tile = xcd * per + (xcd < extra ? xcd : extra) + (blockIdx.x >> 3);
   const int m0 = (tile / tiles_n) * BM, n0 = (tile % tiles_n) * BN;
   const int m1 = m0 + BM < sg.M ? m0 + BM : sg.M;
+  const bool busy = n0 + wn * NI * 32 < Nn;           // a wave without outputs loads and waits, and multiplies nothing
+
+  // rows past the end are read as the last one: a row touches its own results alone, and those are not stored
+  const int c = tid & 7, rr = tid >> 3;
+  const char *bx = reinterpret_cast<const char*>(X + m0 * ldx), *bw = reinterpret_cast<const char*>(W + n0 * ldw);
+  uint32_t ox[RX], ow[RW];                            // bytes from the tile's first row: the host keeps these below 2^31
+#pragma unroll
+  for (int j = 0; j < RX; ++j) {
+    const int r = rr + j * (NT / 8);
+    ox[j] = ((uint32_t)(m0 + r < sg.M ? r : sg.M - 1 - m0) * (uint32_t)ldx + c * V) * sizeof(T);
+  }
+#pragma unroll
+  for (int j = 0; j < RW; ++j) {
+    const int r = rr + j * (NT / 8);
+    ow[j] = ((uint32_t)(n0 + r < Nn ? r : Nn - 1 - n0) * (uint32_t)ldw + c * V) * sizeof(T);
+  }
+  uint4 gx[RX], gw[RW];
+  auto fetch = [&](int s) {
+    const size_t k = (size_t)s * 128;
+#pragma unroll
+    for (int j = 0; j < RX; ++j) gx[j] = line_load(reinterpret_cast<const T*>(bx + k + ox[j]));
+#pragma unroll
+    for (int j = 0; j < RW; ++j) gw[j] = line_load(reinterpret_cast<const T*>(bw + k + ow[j]));
+  };
+  auto stash = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < RX; ++j) { const int r = rr + j * (NT / 8); sx[buf][r * 8 + (c ^ (r & 7))] = gx[j]; }
+#pragma unroll
+    for (int j = 0; j < RW; ++j) { const int r = rr + j * (NT / 8); sw[buf][r * 8 + (c ^ (r & 7))] = gw[j]; }
+  };
+  const int full = Kk / KB, rest = Kk - full * KB;
+  if (full > 0) fetch(0);
+  if (tid < BN) sb[tid] = bias != nullptr && n0 + tid < Nn ? (float)bias[n0 + tid] : 0.f;
+  if (rest > 0) {                                     // what is left of the reduction goes first, through the second buffer
+    const size_t k = (size_t)full * 128;
+    const int n = rest - c * V;
+#pragma unroll 1
+    for (int r = rr; r < BM; r += NT / 8) {
+      const uint32_t o = ((uint32_t)(m0 + r < sg.M ? r : sg.M - 1 - m0) * (uint32_t)ldx + c * V) * sizeof(T);
+      sx[1][r * 8 + (c ^ (r & 7))] = line_load(reinterpret_cast<const T*>(bx + k + o), n);
+    }
+#pragma unroll 1
+    for (int r = rr; r < BN; r += NT / 8) {
+      const uint32_t o = ((uint32_t)(n0 + r < Nn ? r : Nn - 1 - n0) * (uint32_t)ldw + c * V) * sizeof(T);
+      sw[1][r * 8 + (c ^ (r & 7))] = line_load(reinterpret_cast<const T*>(bw + k + o), n);
+    }
+  }
+
   f32x16 acc[NI][MI];
 #pragma unroll
   for (int n = 0; n < NI; ++n)
@@ -264,8 +365,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[n][m][j] = 0.f;
 
-  if (lr.t != nullptr) {
+  if (lr.t != nullptr && busy) {
     const T* b = static_cast<const T*>(lr.b);
+    const bool whole = lr.rank % V == 0;
     int q = seg_find(sg, m0);
     for (q = q < 0 ? 0 : q; q < sg.S && sg.row_start[q] < m1; ++q) {
       const Span sp = seg_span(sg, q, m0, m1);
@@ -275,38 +377,43 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
       for (int m = 0; m < MI; ++m) {
         const int row = m0 + (wm * MI + m) * 32 + l32;
         const bool mine = row >= sp.lo && row < sp.hi;
-        if (__ballot(mine) == 0) continue;
-        const float* tr = lr.t + (long long)(mine ? row : sp.lo) * lr.rank;
-        f32x16 add[NI];
+        if (__ballot(mine) != 0) {
+          const float* tr = lr.t + (long long)(mine ? row : sp.lo) * lr.ldt;
+          f32x16 add[NI];
 #pragma unroll
-        for (int n = 0; n < NI; ++n)
+          for (int n = 0; n < NI; ++n)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) add[n][j] = 0.f;
-        for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
-          const int i = i0 + V * h;
-          Line<T> hi, lo;
+            for (int j = 0; j < 16; ++j) add[n][j] = 0.f;
+#pragma unroll 1
+          for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
+            const int i = i0 + V * h;                 // at most ldt - 8 + V: a half that lies behind the rank reads the other's
+            const bool in = i < lr.rank;
+            f32x4 t4[V / 4];
+            Line<T> hi, lo;
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float v = i + j < lr.rank ? tr[i + j] : 0.f;
-            hi.v[j] = (T)v;
-            const float f = (float)hi.v[j];
-            lo.v[j] = (T)(fabsf(f) < INFINITY ? v - f : 0.f);
+            for (int j = 0; j < V / 4; ++j) t4[j] = *reinterpret_cast<const f32x4*>(tr + (in ? i : i0) + 4 * j);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const float v = in ? t4[j / 4][j % 4] : 0.f;
+              hi.v[j] = (T)v;
+              const float f = (float)hi.v[j];
+              lo.v[j] = (T)(fabsf(f) < INFINITY ? v - f : 0.f);
+            }
+#pragma unroll
+            for (int n = 0; n < NI; ++n) {
+              const int col = n0 + (wn * NI + n) * 32 + l32;
+              const T* bp = ba + (col < Nn ? col : Nn - 1) * lr.sn;
+              uint4 bf = whole ? line_load(bp + (in ? i : i0)) : line_load(bp + i, lr.rank - i);
+              if (!in) bf = uint4{0, 0, 0, 0};
+              add[n] = mma32(bf, __builtin_bit_cast(uint4, hi), add[n], T());
+              if (sizeof(T) == 2) add[n] = mma32(bf, __builtin_bit_cast(uint4, lo), add[n], T());
+            }
           }
 #pragma unroll
-          for (int n = 0; n < NI; ++n) {
-            const int col = n0 + (wn * NI + n) * 32 + l32;
-            Line<T> b8;
+          for (int n = 0; n < NI; ++n)
 #pragma unroll
-            for (int j = 0; j < V; ++j) b8.v[j] = col < Nn && i + j < lr.rank ? ba[col * lr.sn + (i + j) * lr.si] : (T)0.f;
-            const uint4 bf = __builtin_bit_cast(uint4, b8);
-            add[n] = mma32(bf, __builtin_bit_cast(uint4, hi), add[n], T());
-            if (sizeof(T) == 2) add[n] = mma32(bf, __builtin_bit_cast(uint4, lo), add[n], T());
-          }
+            for (int j = 0; j < 16; ++j) acc[n][m][j] = mine ? add[n][j] : acc[n][m][j];
         }
-#pragma unroll
-        for (int n = 0; n < NI; ++n)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) acc[n][m][j] = mine ? add[n][j] : acc[n][m][j];
       }
     }
     if (DROP) {                                       // the mask of x on the low-rank part of dx
@@ -329,85 +436,88 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
     }
   }
 
-  const int c = tid & 7, rr = tid >> 3;
-  uint4 gx[RX], gw[RW];
-  const int steps = (Kk + KB - 1) / KB;
-  auto fetch = [&](int s) {
-    const int k = s * KB + c * V, n = Kk - k;
+  const int rx = (wm * MI * 32 + l32) * 8, rw = (wn * NI * 32 + l32) * 8, sel = l32 & 7;    // rows of a block differ by 32: one XOR
+  auto chunk = [&](int buf, int kk) {                 // 2 V values of the reduction
+    uint4 fx[MI], fw[NI];
+    const int at = (2 * kk + h) ^ sel;
 #pragma unroll
-    for (int j = 0; j < RX; ++j) {
-      const int row = m0 + rr + j * (NT / 8);
-      gx[j] = line_load(X + row * ldx + k, row < sg.M ? n : 0);
-    }
+    for (int m = 0; m < MI; ++m) fx[m] = sx[buf][rx + m * 256 + at];
 #pragma unroll
-    for (int j = 0; j < RW; ++j) {
-      const int row = n0 + rr + j * (NT / 8);
-      gw[j] = line_load(W + row * ldw + k, row < Nn ? n : 0);
-    }
+    for (int n = 0; n < NI; ++n) fw[n] = sw[buf][rw + n * 256 + at];
+#pragma unroll
+    for (int n = 0; n < NI; ++n)
+#pragma unroll
+      for (int m = 0; m < MI; ++m) acc[n][m] = mma32(fw[n], fx[m], acc[n][m], T());
   };
-  auto stash = [&](int buf) {
-#pragma unroll
-    for (int j = 0; j < RX; ++j) { const int r = rr + j * (NT / 8); sx[buf][r * 8 + (c ^ (r & 7))] = gx[j]; }
-#pragma unroll
-    for (int j = 0; j < RW; ++j) { const int r = rr + j * (NT / 8); sw[buf][r * 8 + (c ^ (r & 7))] = gw[j]; }
-  };
-  if (steps > 0) {
-    fetch(0);
+  if (full > 0) {
     stash(0);
-    if (steps > 1) fetch(1);
+    if (full > 1) fetch(1);
+  }
+  __syncthreads();
+  if (rest > 0) {
+    if (busy) {
+#pragma unroll 1
+      for (int kk = 0; kk * 2 * V < rest; ++kk) chunk(1, kk);
+    }
     __syncthreads();
   }
-  for (int s = 0; s < steps; ++s) {
+  for (int s = 0; s < full; ++s) {
     const int buf = s & 1;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint4 fx[MI], fw[NI];
-#pragma unroll
-      for (int m = 0; m < MI; ++m) { const int r = (wm * MI + m) * 32 + l32; fx[m] = sx[buf][r * 8 + ((2 * kk + h) ^ (r & 7))]; }
-#pragma unroll
-      for (int n = 0; n < NI; ++n) { const int r = (wn * NI + n) * 32 + l32; fw[n] = sw[buf][r * 8 + ((2 * kk + h) ^ (r & 7))]; }
-#pragma unroll
-      for (int n = 0; n < NI; ++n)
-#pragma unroll
-        for (int m = 0; m < MI; ++m) acc[n][m] = mma32(fw[n], fx[m], acc[n][m], T());
-    }
-    if (s + 1 < steps) {
+    if (s + 1 < full) {
       stash(buf ^ 1);
-      if (s + 2 < steps) fetch(s + 2);
+      if (s + 2 < full) fetch(s + 2);
+    }
+    if (busy) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) chunk(buf, kk);
     }
     __syncthreads();
   }
+  if (!busy) return;
 
+  // results go out through the wave's own part of the LDS, 32 rows at a time, so that a row leaves in whole lines
+  constexpr int LD = NI * 32 * sizeof(T) / 16 + 1, PER = NI * 32 / V;       // 16-byte units of a row: with one of padding, and stored
+  static_assert(WGM * WGN * 32 * LD <= 2 * (BM + BN) * 8 && 64 % PER == 0, "");
+  uint4* mine = lds + w * 32 * LD;
+  const int cw = n0 + wn * NI * 32;
 #pragma unroll
-  for (int n = 0; n < NI; ++n) {
-    const int cb = n0 + (wn * NI + n) * 32;
+  for (int m = 0; m < MI; ++m) {
+    const int rb = m0 + (wm * MI + m) * 32;
+    if (rb >= sg.M) break;
 #pragma unroll
-    for (int j4 = 0; j4 < 4; ++j4) {
-      const int col = cb + 8 * j4 + 4 * h;
-      float bv[4];
+    for (int n = 0; n < NI; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bv[j] = bias != nullptr && col + j < Nn ? (float)bias[col + j] : 0.f;
+      for (int j4 = 0; j4 < 4; ++j4) {
+        const int col = n * 32 + 8 * j4 + 4 * h;
+        struct alignas(4 * sizeof(T)) P { T v[4]; } p;
 #pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        const int row = m0 + (wm * MI + m) * 32 + l32;
-        if (row >= sg.M) continue;
-        T* o = out + row * ldo + col;
-        struct alignas(sizeof(T)) P { T v[4]; } p;
+        for (int j = 0; j < 4; ++j) p.v[j] = (T)(acc[n][m][4 * j4 + j] + sb[wn * NI * 32 + col + j]);
+        *reinterpret_cast<P*>(reinterpret_cast<T*>(mine + l32 * LD) + col) = p;
+      }
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p.v[j] = (T)(acc[n][m][4 * j4 + j] + bv[j]);
-        if (col + 4 <= Nn) {
-          *reinterpret_cast<P*>(o) = p;
+    for (int i = 0; i < 32 * PER / 64; ++i) {
+      const int r = i * (64 / PER) + lane / PER, u = lane % PER, col = cw + u * V;
+      const Line<T> v = __builtin_bit_cast(Line<T>, mine[r * LD + u]);
+      T* o = out + (long long)(rb + r) * ldo + col;
+      if (rb + r < sg.M) {
+        if (col + V <= Nn) {
+          LooseLine<T> x;
+#pragma unroll
+          for (int j = 0; j < V; ++j) x.v[j] = v.v[j];
+          *reinterpret_cast<LooseLine<T>*>(o) = x;
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) if (col + j < Nn) o[j] = p.v[j];
+          for (int j = 0; j < V; ++j) if (col + j < Nn) o[j] = v.v[j];
         }
       }
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // ---- few rows (M <= 64): the weights are read once, sixteen outputs a workgroup, its waves share the reduction
-constexpr int FEW_ROWS = 64, FEW_WAVES = 8;
+constexpr int FEW_ROWS = 64, FEW_WAVES = 8, FEW_AHEAD = 4;
 
 template <typename T, int MT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ W,
@@ -415,18 +525,40 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restr
                                                                 T* __restrict__ out, long long ldo) {
   __shared__ f32x4 red[FEW_WAVES][MT][64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, steps = (K + 31) >> 5;
+  const int n0 = blockIdx.x * 16, full = K >> 5;
   f32x4 acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = w; s < steps; s += FEW_WAVES) {
-    const int k = 32 * s + 8 * g, n = K - k;
-    const Frag8<T> a = frag_load(W + (n0 + l16) * ldw + k, n0 + l16 < N ? n : 0);
+  const T *wp = W + (n0 + l16 < N ? n0 + l16 : N - 1) * ldw + 8 * g, *xp[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int row = 16 * m + l16;
-      acc[m] = mma16(a, frag_load(X + row * ldx + k, row < sg.M ? n : 0), acc[m]);
+  for (int m = 0; m < MT; ++m) xp[m] = X + (16 * m + l16 < sg.M ? 16 * m + l16 : sg.M - 1) * ldx + 8 * g;
+  int s = w;
+  for (; s + FEW_WAVES * (FEW_AHEAD - 1) < full; s += FEW_WAVES * FEW_AHEAD) {
+    Frag8<T> a[FEW_AHEAD], x[FEW_AHEAD][MT];
+#pragma unroll
+    for (int u = 0; u < FEW_AHEAD; ++u) {
+      a[u] = frag_load(wp + 32 * (s + FEW_WAVES * u));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[u][m] = frag_load(xp[m] + 32 * (s + FEW_WAVES * u));
     }
+#pragma unroll
+    for (int u = 0; u < FEW_AHEAD; ++u)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m] = mma16(a[u], x[u][m], acc[m]);
+  }
+  for (; s < full; s += FEW_WAVES) {
+    const Frag8<T> a = frag_load(wp + 32 * s);
+    Frag8<T> x[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) x[m] = frag_load(xp[m] + 32 * s);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = mma16(a, x[m], acc[m]);
+  }
+  if (K > 32 * full && w == full % FEW_WAVES) {
+    const int n = K - 32 * full - 8 * g;
+    const Frag8<T> a = frag_load(wp + 32 * full, n);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = mma16(a, frag_load(xp[m] + 32 * full, n), acc[m]);
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m) red[w][m][lane] = acc[m];
@@ -446,10 +578,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restr
   if (a >= 0) {
     const T* b = static_cast<const T*>(lr.b) + (long long)a * lr.sa;
     for (int i = 0; i < lr.rank; ++i) {
-      const float ti = lr.t[(long long)row * lr.rank + i];
+      const float ti = lr.t[(long long)row * lr.ldt + i];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (col + j < N) v[j] = fmaf(ti, (float)b[(col + j) * lr.sn + i * lr.si], v[j]);
+        if (col + j < N) v[j] = fmaf(ti, (float)b[(col + j) * lr.sn + i], v[j]);
     }
   }
   if (row < sg.M) {
@@ -462,26 +594,59 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restr
 // ---- sums over rows: G_a[p][i] = sum over the rows m of adapter a of X[m][p] t[m][i], 128 columns p and up to 64 ranks a
 // workgroup.  The reduction runs along the rows, so both operands are read as they lie: 16 x 16 x 4 fp32 products, lane (p, m).
 // The fp32 matrix rate is above what reading X needs up to a rank of 16 and keeps t exact.
-constexpr int OU_COLS = 128;
+constexpr int OU_COLS = 128, OU_AHEAD = 4;
 
 // adds rows [lo, hi) to the sums of the four waves: wave w takes four rows of every sixteen
 template <typename T, int RT>
-__device__ __forceinline__ void outer_rows(f32x4 (&acc)[8][RT], const T* X, long long ldx, int P, const float* t, int rank, int ib,
+__device__ __forceinline__ void outer_rows(f32x4 (&acc)[8][RT], const T* X, long long ldx, int P, const float* t, int rank, int ldt, int ib,
                                            int p, int lo, int hi, int w, int lane, bool drop, const KeepArgs& ka, KeepKey key) {
   const int l16 = lane & 15, g = lane >> 4;
-  for (int m0 = lo + 4 * w; m0 < hi; m0 += 16) {
-    const int m = m0 + g;
-    const bool in = m < hi;
-    Frag8<T> x = frag_load(X + (long long)(in ? m : lo) * ldx + p, in ? P - p : 0);
-    if (drop) frag_keep(x, keep8(ka, key, (uint64_t)m, (uint32_t)(p >> 3)));
+  int at[RT];                                          // ranks past the rank are read as the last one: not stored
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int ri = ib + 16 * i + l16;
-      const float tv = in && ri < rank ? t[(long long)m * rank + ri] : 0.f;
+  for (int i = 0; i < RT; ++i) at[i] = ib + 16 * i + l16 < ldt ? ib + 16 * i + l16 : ldt - 1;
+  auto step = [&](Frag8<T> x, const float (&tv)[RT], int m) {
+    if (drop) {
+      uint32_t keep = keep8(ka, key, (uint64_t)m, (uint32_t)(p >> 3));
+      if (p & 7) keep = (keep | keep8(ka, key, (uint64_t)m, (uint32_t)(p >> 3) + 1) << 8) >> (p & 7);
+      frag_keep(x, keep);
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[j], tv, acc[j][i], 0, 0, 0);
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[j], tv[i], acc[j][i], 0, 0, 0);
+  };
+  int m0 = lo + 4 * w;
+  if (P >= 8) {
+    for (; m0 + 16 * (OU_AHEAD - 1) + 4 <= hi; m0 += 16 * OU_AHEAD) {          // the loads of sixteen rows in flight
+      Frag8<T> x[OU_AHEAD];
+      float tv[OU_AHEAD][RT];
+#pragma unroll
+      for (int u = 0; u < OU_AHEAD; ++u) {
+        const long long m = m0 + 16 * u + g;
+        x[u] = frag_load(X + m * ldx + p);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) tv[u][i] = t[m * ldt + at[i]];
+      }
+#pragma unroll
+      for (int u = 0; u < OU_AHEAD; ++u) step(x[u], tv[u], m0 + 16 * u + g);
     }
   }
+  for (; m0 < hi; m0 += 16) {
+    const int m = m0 + g;
+    const bool in = m < hi;
+    const T* xr = X + (long long)(in ? m : lo) * ldx + p;
+    const Frag8<T> x = frag_load(xr, in ? P - p : 0);
+    float tv[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) tv[i] = in ? t[(long long)m * ldt + at[i]] : 0.f;
+    step(x, tv, m);
+  }
+}
+
+// first of the eight columns of a lane: the last lanes of a row share its last eight (they come to the same bits)
+__device__ __forceinline__ int outer_col(int P, int pb, int l16) {
+  const int p = pb * OU_COLS + 8 * l16;
+  return p + 8 <= P || P < 8 ? p : P - 8;
 }
 
 // one job of the sums: dA (X = x, t = u) or dB (X = dy, t = t)
@@ -490,6 +655,7 @@ struct Outer {
   long long ldx;
   int P;                   // columns
   const float* t;
+  int ldt;
   void* out;               // element (a, p, i) at a * oa + p * op + i * oi
   long long oa, op, oi;
   float* part;             // [slot][column block][rank chunk][tile (j, i)][lane] f32x4
@@ -502,14 +668,14 @@ template <int RT> __device__ __forceinline__ size_t part_at(const Outer& o, int 
   return (((size_t)slot * o.blocks + pb) * chunks + rc) * (8 * RT * 64);
 }
 
-// value q of tile (j, i) in `lane`: column pb * 128 + 8 (4 (lane / 16) + q) + j, rank ib + 16 i + lane % 16
+// value q of tile (j, i) in `lane`: column outer_col(4 (lane / 16) + q) + j, rank ib + 16 i + lane % 16
 template <typename T, int RT>
 __device__ __forceinline__ void outer_store(const Outer& o, f32x4 v, int tile, int lane, int a, int pb, int ib, int rank) {
   const int j = tile / RT, i = ib + 16 * (tile % RT) + (lane & 15);
   if (i >= rank) return;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const int p = pb * OU_COLS + 8 * (4 * (lane >> 4) + q) + j;
+    const int p = outer_col(o.P, pb, 4 * (lane >> 4) + q) + j;
     if (p < o.P) static_cast<T*>(o.out)[a * o.oa + p * o.op + i * o.oi] = (T)(v[q] * o.factor);
   }
 }
@@ -532,7 +698,7 @@ __device__ __forceinline__ void outer_run(const Outer& o, const Segs& sg, const 
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int i = 0; i < RT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      outer_rows<T, RT>(acc, static_cast<const T*>(o.X), o.ldx, o.P, o.t, rank, 64 * rc, pb * OU_COLS + 8 * l16, sp.lo, sp.hi, w, lane, o.drop != 0, ka, key);
+      outer_rows<T, RT>(acc, static_cast<const T*>(o.X), o.ldx, o.P, o.t, rank, o.ldt, 64 * rc, outer_col(o.P, pb, l16), sp.lo, sp.hi, w, lane, o.drop != 0, ka, key);
       f32x4* to = reinterpret_cast<f32x4*>(o.part) + part_at<RT>(o, run + q, pb, rc, chunks);
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
@@ -619,8 +785,8 @@ __global__ __launch_bounds__(256) void k_outer_direct(Outer oa, Outer ob, Segs s
       const int q = list.q[e];
       const int lo = sg.row_start[q] > 0 ? sg.row_start[q] : 0, hi = sg.row_start[q + 1] < sg.M ? sg.row_start[q + 1] : sg.M;
       const T* X = static_cast<const T*>(o.X);
-      const int p = pb * OU_COLS + 8 * l16;
-      outer_rows<T, RT>(acc, X, o.ldx, o.P, o.t, rank, ib, p, lo, hi, w, lane, o.drop != 0, ka, key);
+      const int p = outer_col(o.P, pb, l16);
+      outer_rows<T, RT>(acc, X, o.ldx, o.P, o.t, rank, o.ldt, ib, p, lo, hi, w, lane, o.drop != 0, ka, key);
     }
   }
 #pragma unroll
@@ -651,13 +817,14 @@ __global__ __launch_bounds__(256) void k_turn(const T* __restrict__ in, long lon
 
 // ---- host side
 
+int pad8(int v) { return (v + 7) & ~7; }
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 size_t type_size(int type) { return type == HM_TYPE_F32 ? 4 : 2; }
 
 struct Plan {
   int rt, chunks, rows_per_run, runs, direct;
-  long long npad;
-  size_t wt, bt, u, pa, pb, total;       // offsets into the workspace
+  long long npad, rpad;
+  size_t wt, bt, at, u, pa, pb, total;       // offsets into the workspace
 };
 
 constexpr size_t MAX_PART = size_t(512) << 20;
@@ -677,12 +844,14 @@ Plan make_plan(const hm_adapter_args& g) {
   p.rows_per_run = (int)per;
   p.runs = (int)((g.rows + per - 1) / per);
   p.npad = (g.n + 7) & ~7ll;
+  p.rpad = pad8(g.rank);
   const size_t slot = (size_t)p.chunks * 8 * p.rt * 64 * sizeof(f32x4), slots = (size_t)p.runs + g.segments;
   p.direct = slots * slot * (ba + bb) > MAX_PART;
   size_t at = 0;
   p.wt = at; at = up256(at + (size_t)g.k * p.npad * type_size(g.type));
   p.bt = at; at = up256(at + (size_t)g.adapters * g.rank * p.npad * type_size(g.type));
-  p.u = at;  at = up256(at + (size_t)g.rows * g.rank * sizeof(float));
+  p.at = at; at = up256(at + (size_t)g.adapters * g.k * p.rpad * type_size(g.type));
+  p.u = at;  at = up256(at + (size_t)g.rows * p.rpad * sizeof(float));
   p.pa = at; at = up256(at + (p.direct ? 0 : slots * slot * ba));
   p.pb = at; at = up256(at + (p.direct ? 0 : slots * slot * bb));
   p.total = at;
@@ -709,6 +878,8 @@ int check_args(const char* name, const hm_adapter_args* g, KeepArgs* ka) {
     hm_set_error("%s: null argument", name); return -1; }
   if ((g->rows > 1 && g->ld_x < g->k) || (g->n > 1 && g->ld_w < g->k)) {
     hm_set_error("%s: a row stride is less than k = %d", name, g->k); return -1; }
+  if (g->ld_x > HM_ADAPTER_MAX_STRIDE || g->ld_w > HM_ADAPTER_MAX_STRIDE) {
+    hm_set_error("%s: a row stride is over %d", name, HM_ADAPTER_MAX_STRIDE); return -1; }
   return 0;
 }
 
@@ -726,13 +897,13 @@ int shrink(const hm_adapter_args& g, const T* X, long long ldx, int K, const T* 
   const Segs sg = segs_of(g);
   const float f = drop ? ka.up : 1.f;
   if (few_rows_each(g)) {
-    const long long waves = g.rows * ((g.rank + SR_RANKS - 1) / SR_RANKS);
+    const long long waves = g.rows * (pad8(g.rank) / SR_RANKS);
     const dim3 grid((unsigned)((waves + 3) / 4));
-    if (drop) hipLaunchKernelGGL((k_shrink_rows<T, true>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t);
-    else hipLaunchKernelGGL((k_shrink_rows<T, false>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t);
+    if (drop) hipLaunchKernelGGL((k_shrink_rows<T, true>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t, pad8(g.rank));
+    else hipLaunchKernelGGL((k_shrink_rows<T, false>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t, pad8(g.rank));
   } else {
     const dim3 grid((unsigned)((g.rows + SH_ROWS - 1) / SH_ROWS), (g.rank + SH_RANKS - 1) / SH_RANKS);
-#define HM_GO(RT, D) hipLaunchKernelGGL((k_shrink<T, RT, D>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t)
+#define HM_GO(RT, D) hipLaunchKernelGGL((k_shrink<T, RT, D>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t, pad8(g.rank))
     if (g.rank <= 16) { if (drop) HM_GO(1, true); else HM_GO(1, false); }
     else if (g.rank <= 32) { if (drop) HM_GO(2, true); else HM_GO(2, false); }
     else { if (drop) HM_GO(4, true); else HM_GO(4, false); }
@@ -746,10 +917,13 @@ template <typename T>
 int project(const hm_adapter_args& g, const T* X, long long ldx, int Kk, const T* W, long long ldw, int Nn, const T* bias,
             const LowRank& lr, bool drop, const KeepArgs& ka, T* out, long long ldo, hipStream_t st) {
   const Segs sg = segs_of(g);
-  const long long tm = (g.rows + 127) / 128, tn = (Nn + 127) / 128;
-  const dim3 grid((unsigned)(tm * tn));
-  if (drop) hipLaunchKernelGGL((k_project<T, 128, 128, 2, 2, true>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, (int)tn);
-  else hipLaunchKernelGGL((k_project<T, 128, 128, 2, 2, false>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, (int)tn);
+#define HM_GO(BM, BN, WGM, WGN, D)                                                                                                   \
+  hipLaunchKernelGGL((k_project<T, BM, BN, WGM, WGN, D>), dim3((unsigned)(((g.rows + BM - 1) / BM) * ((Nn + BN - 1) / BN))),         \
+                     dim3(64 * WGM * WGN), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, (Nn + BN - 1) / BN)
+  const long long big = ((g.rows + 255) / 256) * ((Nn + 255) / 256);
+  if (big >= 128) { if (drop) HM_GO(256, 256, 2, 4, true); else HM_GO(256, 256, 2, 4, false); }
+  else { if (drop) HM_GO(128, 128, 2, 2, true); else HM_GO(128, 128, 2, 2, false); }
+#undef HM_GO
   HM_CHECK_HIP(hipGetLastError());
   return 0;
 }
@@ -763,7 +937,7 @@ template <typename T> int forward(const hm_adapter_args& g, const KeepArgs& ka, 
     const int rc = shrink<T>(g, X, g.ld_x, g.k, A, g.k, (long long)g.rank * g.k, ka.threshold != 0, ka, d_t, st);
     if (rc) return rc;
   }
-  const LowRank lr = {any ? d_t : nullptr, g.d_b, (long long)g.n * g.rank, g.rank, 1, g.rank};
+  const LowRank lr = {any ? d_t : nullptr, g.d_b, (long long)g.n * g.rank, g.rank, g.rank, pad8(g.rank)};
   if (g.rows <= FEW_ROWS) {
     const dim3 grid((g.n + 15) / 16);
     const Segs sg = segs_of(g);
@@ -790,7 +964,7 @@ int backward(const hm_adapter_args& g, const KeepArgs& ka, const void* d_dy, lon
              long long ld_dx, void* d_da, void* d_db, char* ws, hipStream_t st) {
   const Plan p = make_plan(g);
   const T *X = static_cast<const T*>(g.d_x), *W = static_cast<const T*>(g.d_w), *dy = static_cast<const T*>(d_dy);
-  T *wt = reinterpret_cast<T*>(ws + p.wt), *bt = reinterpret_cast<T*>(ws + p.bt);
+  T *wt = reinterpret_cast<T*>(ws + p.wt), *bt = reinterpret_cast<T*>(ws + p.bt), *at = reinterpret_cast<T*>(ws + p.at);
   float* u = reinterpret_cast<float*>(ws + p.u);
   const bool any = g.adapters > 0 && g.segments > 0 && g.rows > 0;
   int rc;
@@ -801,14 +975,15 @@ int backward(const hm_adapter_args& g, const KeepArgs& ka, const void* d_dy, lon
   }
   if (d_dx != nullptr && g.rows > 0) {
     if ((rc = turn<T>(W, g.ld_w, 0, g.n, g.k, wt, p.npad, 0, 1, st))) return rc;
-    const LowRank lr = {any ? u : nullptr, g.d_a, (long long)g.rank * g.k, 1, g.k, g.rank};
+    if (any && (rc = turn<T>(static_cast<const T*>(g.d_a), g.k, (long long)g.rank * g.k, g.rank, g.k, at, p.rpad, g.k * p.rpad, g.adapters, st))) return rc;
+    const LowRank lr = {any ? u : nullptr, at, g.k * p.rpad, p.rpad, g.rank, pad8(g.rank)};
     if ((rc = project<T>(g, dy, ld_dy, g.n, wt, p.npad, g.k, nullptr, lr, ka.threshold != 0, ka, static_cast<T*>(d_dx), ld_dx, st))) return rc;
   }
   if (g.adapters > 0 && (d_da != nullptr || d_db != nullptr)) {
     const Segs sg = segs_of(g);
-    Outer oa = {X, g.ld_x, d_da != nullptr ? g.k : 0, u, d_da, (long long)g.rank * g.k, 1, g.k, reinterpret_cast<float*>(ws + p.pa),
+    Outer oa = {X, g.ld_x, d_da != nullptr ? g.k : 0, u, pad8(g.rank), d_da, (long long)g.rank * g.k, 1, g.k, reinterpret_cast<float*>(ws + p.pa),
                 d_da != nullptr ? (g.k + OU_COLS - 1) / OU_COLS : 0, ka.threshold != 0, ka.up};
-    Outer ob = {dy, ld_dy, d_db != nullptr ? g.n : 0, d_t, d_db, (long long)g.n * g.rank, g.rank, 1, reinterpret_cast<float*>(ws + p.pb),
+    Outer ob = {dy, ld_dy, d_db != nullptr ? g.n : 0, d_t, pad8(g.rank), d_db, (long long)g.n * g.rank, g.rank, 1, reinterpret_cast<float*>(ws + p.pb),
                 d_db != nullptr ? (g.n + OU_COLS - 1) / OU_COLS : 0, 0, 1.f};
     const int blocks = oa.blocks > ob.blocks ? oa.blocks : ob.blocks;
 #define HM_GO(RT)                                                                                                                    \
@@ -862,6 +1037,7 @@ extern "C" int hm_adapter_linear_backward(const hm_adapter_args* g, const void* 
     hm_set_error("hm_adapter_linear_backward: null argument"); return -1; }
   if (g->rows > 1 && (ld_dy < g->n || (d_dx != nullptr && ld_dx < g->k))) {
     hm_set_error("hm_adapter_linear_backward: a row stride is less than the columns"); return -1; }
+  if (ld_dy > HM_ADAPTER_MAX_STRIDE) { hm_set_error("hm_adapter_linear_backward: a row stride is over %d", HM_ADAPTER_MAX_STRIDE); return -1; }
   const Plan p = make_plan(*g);
   if (d_ws == nullptr || ws_bytes < (long long)p.total) {
     hm_set_error("hm_adapter_linear_backward: workspace of %lld bytes, %lld are needed", d_ws == nullptr ? 0ll : ws_bytes, (long long)p.total); return -1; }

@@ -178,7 +178,7 @@ def _adapter_forward(x, weight, bias, A, B, scale, row_start, adapter, draws):
     args = _adapter_args(x, weight, bias, A, B, scale, row_start, adapter, draws)
     n = weight.shape[0]
     y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    t = torch.empty(args.rows, args.rank, dtype=torch.float32, device=x.device)
+    t = torch.empty(args.rows, (args.rank + 7) // 8 * 8, dtype=torch.float32, device=x.device)
     guard, stream = _on(x.device)
     with guard:
         _lib.check(_lib.lib().hm_adapter_linear(ctypes.byref(args), y.data_ptr(), n, t.data_ptr(), stream), "hm_adapter_linear")

@@ -369,6 +369,7 @@ int hm_dropout_backward(const void* d_dy, long long ld_dy, const void* d_y, long
 #define HM_ADAPTER_MAX_ROWS 16777216
 #define HM_ADAPTER_MAX_WIDTH 65536
 #define HM_ADAPTER_MAX_RANK 256
+#define HM_ADAPTER_MAX_STRIDE 2097152   /* elements between rows of x, w and dy */
 #define HM_ADAPTER_MAX_COUNT 65535
 typedef struct hm_adapter_args {
   int type;                /* HM_TYPE_* of x, w, bias, a, b and of the results                       */
@@ -392,8 +393,8 @@ typedef struct hm_adapter_args {
   unsigned long long row0;
 } hm_adapter_args;
 
-/* d_t [rows][rank] floats: scale[a] drop(x) A[a]^T / (1 - p) of the rows that have an adapter; scratch, and what the backward pass
- * reads.  Not used (may be NULL) when adapters or segments is 0. */
+/* d_t [rows][rank rounded up to 8] floats, 16-byte aligned: scale[a] drop(x) A[a]^T / (1 - p) of the rows that have an adapter;
+ * scratch, and what the backward pass reads.  Not used (may be NULL) when adapters or segments is 0. */
 int hm_adapter_linear(const hm_adapter_args* args, void* d_y, long long ld_y, float* d_t, void* stream);
 /* Gradients, each where its pointer is not NULL: d_dx [rows][k], d_da like a, d_db like b (zeros for an adapter without rows).
  * The projection and the scales get none.  d_ws: workspace of at least hm_adapter_linear_backward_bytes(args) bytes (-1 on an

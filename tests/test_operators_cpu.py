@@ -58,7 +58,7 @@ def args(**kw):
     (dict(rank=0), b"rank"), (dict(rank=257), b"rank"), (dict(adapters=-1), b"adapters"), (dict(segments=-1), b"requests"),
     (dict(adapters=70000), b"adapters"), (dict(p=-0.1), b"p must"), (dict(p=1.5), b"p must"), (dict(p=float("nan")), b"p must"),
     (dict(d_x=0), b"null"), (dict(d_w=0), b"null"), (dict(d_a=0), b"null"), (dict(d_row_start=0), b"null"), (dict(d_adapter=0), b"null"),
-    (dict(ld_x=7), b"stride"), (dict(ld_w=7), b"stride")])
+    (dict(ld_x=7), b"stride"), (dict(ld_w=7), b"stride"), (dict(ld_x=1 << 22), b"stride"), (dict(ld_w=1 << 22), b"stride")])
 def test_adapter_entries_refuse(kw, word):
     lib, a = _lib.lib(), args(**kw)
     assert lib.hm_adapter_linear(ctypes.byref(a), 4096, 8, 4096, None) < 0 and word in lib.hm_last_error()
