@@ -8,10 +8,10 @@
 // x (M, K), W (N, K), A (adapters, r, K), B (adapters, N, r).  Request q has the rows row_start[q] .. row_start[q + 1] - 1 and
 // the adapter adapter[q]; a value outside 0 .. adapters - 1, or no request at all, leaves the bare projection.
 //
-// Arithmetic: every sum is held in 32 bits.  t and u stay in 32 bits in memory; where they meet 16-bit weights on the matrix
-// cores they are split into a high and a low 16-bit part (two products: the rank is small), so they add no rounding.  A value
-// kept by the dropout is NOT multiplied by 1 / (1 - p) before the product (that would round it): the factor joins s_a.
-// fp16: |t| or |u| beyond 65504 overflows to infinity.
+// Arithmetic: every sum is held in 32 bits.  t and u stay in 32 bits in memory; where they meet 16-bit operands on the matrix
+// cores they are split into a high and a low bf16 part (off by 2^-17 of themselves; fp32's range, so nothing overflows or goes
+// under), and an fp16 operand there into two bf16 parts, which is exact (11 = 8 + 3 bits).  A value kept by the dropout is NOT
+// multiplied by 1 / (1 - p) before the product (that would round it): the factor joins s_a.
 //
 // A row's result depends on its own row and its own adapter alone: a lane of a matrix product holds one row (rows are the
 // columns of the MFMA), and what another request's adapter adds is selected away, not multiplied by 0 -- an infinity or NaN in
@@ -79,6 +79,18 @@ __device__ __forceinline__ f32x4 mma16(const Frag8<float>& a, const Frag8<float>
   return c;
 }
 
+// keeps the scheduler from spreading a group of loads between the products that wait for them, which it does to save registers:
+// these kernels live from the loads in flight
+__device__ __forceinline__ void all_loads_first() { __builtin_amdgcn_sched_barrier(0); }
+
+// what a lane of this wave wrote to the LDS is there for its other lanes: LDS accesses of a wave keep their order, so only the
+// compiler has to be held
+__device__ __forceinline__ void wave_sees_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // p[0 .. 7], of which the first n exist (n <= 0: none): zero where nothing is
 template <typename T> __device__ __forceinline__ Frag8<T> frag_load(const T* p, int n) {
   Frag8<T> f;
@@ -104,19 +116,111 @@ template <typename T> __device__ __forceinline__ void frag_keep(Frag8<T>& f, uin
   for (int j = 0; j < 8; ++j) f.v[j] = (keep >> j) & 1 ? f.v[j] : (T)0.f;
 }
 
-// ---- t / u: 32 rows x up to 64 ranks per workgroup, the four waves share the reduction.  Bound by reading X once.
-constexpr int SH_ROWS = 32, SH_RANKS = 64, SH_AHEAD = 4;
+// ---- lines of 128 bytes along the reduction: what a row of an LDS tile holds
+template <typename T> struct Lines { static constexpr int V = 16 / sizeof(T), KB = 128 / sizeof(T); };
+template <typename T> struct alignas(16) Line { T v[16 / sizeof(T)]; };
+template <typename T> struct alignas(sizeof(T)) LooseLine { T v[16 / sizeof(T)]; };     // the same at the alignment of one value
 
-template <typename T, int RT, bool DROP>
-__global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ R, long long ldr,
-                                                long long stride_a, int rank, float factor, Segs sg, KeepArgs ka,
-                                                float* __restrict__ t, int ldt) {
-  __shared__ f32x4 red[4][2 * RT][64];
+template <typename T> __device__ __forceinline__ uint4 line_load(const T* p) {
+  return __builtin_bit_cast(uint4, *reinterpret_cast<const LooseLine<T>*>(p));
+}
+// the first n values of a line (n <= 0: none), zero behind them
+template <typename T> __device__ __forceinline__ uint4 line_load(const T* p, int n) {
+  constexpr int V = Lines<T>::V;
+  if (n >= V) return line_load(p);
+  Line<T> o;
+#pragma unroll
+  for (int j = 0; j < V; ++j) o.v[j] = j < n ? p[j] : (T)0.f;
+  return __builtin_bit_cast(uint4, o);
+}
+
+// ---- thin products: a wave's share of A (up to 64 rows) times B^T (up to 64 rows), lines w, w + NW, .. of the reduction.  Every
+// wave stages its own lines in its own part of the LDS -- global memory sees whole lines (64-byte pieces of rows that lie a power
+// of two apart come from few channels and take four times as long), no wave waits for another -- and has the next line's loads
+// in flight while it multiplies.
+template <int AT, int BT> constexpr int strip_units() { return (AT + BT) * 128; }       // 16-byte units of LDS a wave
+
+template <typename T, int AT, int BT, int NW, bool DROP>
+__device__ __forceinline__ void strip_sum(f32x4 (&acc)[BT][AT], const T* A, long long lda, int na, const T* B, long long ldb, int nb, int K,
+                                          uint4* own, int w, int lane, const KeepArgs& ka, KeepKey key, int row0) {
+  constexpr int V = Lines<T>::V, KB = Lines<T>::KB;
+  const int l16 = lane & 15, g = lane >> 4, c = lane & 7, r8 = lane >> 3;
+  const char *ba = reinterpret_cast<const char*>(A), *bb = reinterpret_cast<const char*>(B);
+  // rows past the end are read as the last one: a row of A or B touches its own results alone
+  uint32_t oa[2 * AT], ob[2 * BT];
+#pragma unroll
+  for (int i = 0; i < 2 * AT; ++i) { const int r = 8 * i + r8; oa[i] = ((uint32_t)(r < na ? r : na - 1) * (uint32_t)lda + c * V) * sizeof(T); }
+#pragma unroll
+  for (int i = 0; i < 2 * BT; ++i) { const int r = 8 * i + r8; ob[i] = ((uint32_t)(r < nb ? r : nb - 1) * (uint32_t)ldb + c * V) * sizeof(T); }
+  const int full = K / KB, lines = (K + KB - 1) / KB;
+  uint4 ga[2 * AT], gb[2 * BT];
+  auto fetch = [&](int s) {
+    const size_t k = (size_t)s * 128;
+    if (s < full) {
+#pragma unroll
+      for (int i = 0; i < 2 * BT; ++i) gb[i] = line_load(reinterpret_cast<const T*>(bb + k + ob[i]));
+#pragma unroll
+      for (int i = 0; i < 2 * AT; ++i) ga[i] = line_load(reinterpret_cast<const T*>(ba + k + oa[i]));
+    } else {
+      const int n = K - s * KB - c * V;
+#pragma unroll
+      for (int i = 0; i < 2 * BT; ++i) gb[i] = line_load(reinterpret_cast<const T*>(bb + k + ob[i]), n);
+#pragma unroll
+      for (int i = 0; i < 2 * AT; ++i) ga[i] = line_load(reinterpret_cast<const T*>(ba + k + oa[i]), n);
+    }
+  };
+  auto frag = [&](int row, int kk) {
+    Frag8<T> f;
+    if constexpr (sizeof(T) == 2) {
+      f.v = __builtin_bit_cast(decltype(f.v), own[row * 8 + ((4 * kk + g) ^ (row & 7))]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 v = __builtin_bit_cast(f32x4, own[row * 8 + ((2 * g + h) ^ (row & 7))]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.v[4 * h + j] = v[j];
+      }
+    }
+    return f;
+  };
+  if (w < lines) fetch(w);
+  for (int s = w; s < lines; s += NW) {
+#pragma unroll
+    for (int i = 0; i < 2 * AT; ++i) { const int r = 8 * i + r8; own[r * 8 + (c ^ (r & 7))] = ga[i]; }
+#pragma unroll
+    for (int i = 0; i < 2 * BT; ++i) { const int r = 16 * AT + 8 * i + r8; own[r * 8 + (c ^ (r & 7))] = gb[i]; }
+    if (s + NW < lines) fetch(s + NW);
+    wave_sees_lds();
+#pragma unroll
+    for (int kk = 0; kk < KB / 32; ++kk) {
+      Frag8<T> a[AT];
+#pragma unroll
+      for (int i = 0; i < AT; ++i) a[i] = frag(16 * i + l16, kk);
+#pragma unroll
+      for (int m = 0; m < BT; ++m) {
+        Frag8<T> x = frag(16 * AT + 16 * m + l16, kk);
+        if (DROP) frag_keep(x, keep8(ka, key, (uint64_t)(row0 + 16 * m + l16), (uint32_t)((s * KB + 32 * kk + 8 * g) >> 3)));
+#pragma unroll
+        for (int i = 0; i < AT; ++i) acc[m][i] = mma16(a[i], x, acc[m][i]);
+      }
+    }
+    wave_sees_lds();
+  }
+}
+
+// ---- t / u: 32 rows x up to 64 ranks a workgroup, its waves share the reduction.  Bound by reading X once.
+constexpr int SH_ROWS = 32, SH_RANKS = 64;
+
+template <typename T, int RT, int NW, bool DROP>
+__global__ __launch_bounds__(64 * NW) void k_shrink(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ R, long long ldr,
+                                                    long long stride_a, int rank, float factor, Segs sg, KeepArgs ka,
+                                                    float* __restrict__ t, int ldt) {
+  constexpr int U = strip_units<RT, 2>();
+  __shared__ uint4 lds[NW * U];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
   const int r0 = blockIdx.x * SH_ROWS, ib = blockIdx.y * SH_RANKS;
   const int r1 = r0 + SH_ROWS < sg.M ? r0 + SH_ROWS : sg.M;
   const KeepKey key = keep_key(ka);
-  const int full = K >> 5;
   int q = seg_find(sg, r0);
   for (q = q < 0 ? 0 : q; q < sg.S && sg.row_start[q] < r1; ++q) {
     const Span sp = seg_span(sg, q, r0, r1);
@@ -126,72 +230,24 @@ __global__ __launch_bounds__(256) void k_shrink(const T* __restrict__ X, long lo
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int i = 0; i < RT; ++i) acc[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // rows past the end and ranks past the rank are read as the last one: they touch their own results alone
-    const T *xp[2], *ap[RT];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) { const int row = r0 + 16 * m + l16; xp[m] = X + (row < sg.M ? row : sg.M - 1) * ldx + 8 * g; }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int ri = ib + 16 * i + l16;
-      ap[i] = R + (long long)sp.a * stride_a + (ri < rank ? ri : rank - 1) * ldr + 8 * g;
-    }
-    auto step = [&](const Frag8<T> (&x)[2], const Frag8<T> (&a)[RT], int s) {
-      Frag8<T> xk[2] = {x[0], x[1]};
-      if (DROP) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) frag_keep(xk[m], keep8(ka, key, (uint64_t)(r0 + 16 * m + l16), (uint32_t)(4 * s + g)));
-      }
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) acc[m][i] = mma16(a[i], xk[m], acc[m][i]);
-    };
-    int s = w;
-    for (; s + 4 * (SH_AHEAD - 1) < full; s += 4 * SH_AHEAD) {     // the loads of four steps in flight
-      Frag8<T> x[SH_AHEAD][2], a[SH_AHEAD][RT];
-#pragma unroll
-      for (int u = 0; u < SH_AHEAD; ++u) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) x[u][m] = frag_load(xp[m] + 32 * (s + 4 * u));
-#pragma unroll
-        for (int i = 0; i < RT; ++i) a[u][i] = frag_load(ap[i] + 32 * (s + 4 * u));
-      }
-#pragma unroll
-      for (int u = 0; u < SH_AHEAD; ++u) step(x[u], a[u], s + 4 * u);
-    }
-    for (; s < full; s += 4) {
-      Frag8<T> x[2], a[RT];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) x[m] = frag_load(xp[m] + 32 * s);
-#pragma unroll
-      for (int i = 0; i < RT; ++i) a[i] = frag_load(ap[i] + 32 * s);
-      step(x, a, s);
-    }
-    if (K > 32 * full && w == (full & 3)) {
-      const int n = K - 32 * full - 8 * g;
-      Frag8<T> x[2], a[RT];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) x[m] = frag_load(xp[m] + 32 * full, n);
-#pragma unroll
-      for (int i = 0; i < RT; ++i) a[i] = frag_load(ap[i] + 32 * full, n);
-      step(x, a, full);
-    }
+    strip_sum<T, RT, 2, NW, DROP>(acc, R + (long long)sp.a * stride_a + ib * ldr, ldr, rank - ib, X + (long long)r0 * ldx, ldx, sg.M - r0, K,
+                                  lds + w * U, w, lane, ka, key, r0);
+    f32x4* red = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int i = 0; i < RT; ++i) red[w][m * RT + i][lane] = acc[m][i];
+      for (int i = 0; i < RT; ++i) red[w * U + (m * RT + i) * 64 + lane] = acc[m][i];
     __syncthreads();
     const float f = factor * (sg.scale != nullptr ? sg.scale[sp.a] : 1.f);
+    for (int u = w; u < 2 * RT; u += NW) {
+      f32x4 v = red[u * 64 + lane];
 #pragma unroll
-    for (int v4 = 0; v4 < (2 * RT + 3) / 4; ++v4) {
-      const int u = w + 4 * v4;
-      if (u >= 2 * RT) break;
-      const f32x4 v = (red[0][u][lane] + red[1][u][lane]) + (red[2][u][lane] + red[3][u][lane]);
+      for (int o = 1; o < NW; ++o) v += red[o * U + u * 64 + lane];
       const int row = r0 + 16 * (u / RT) + l16, i0 = ib + 16 * (u % RT) + 4 * g;
-      if (row >= sp.lo && row < sp.hi) {
+      if (row >= sp.lo && row < sp.hi && i0 < ldt) {   // ldt is a multiple of 8: four at once
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (i0 + j < ldt) t[(long long)row * ldt + i0 + j] = i0 + j < rank ? v[j] * f : 0.f;
+        for (int j = 0; j < 4; ++j) v[j] = i0 + j < rank ? v[j] * f : 0.f;
+        *reinterpret_cast<f32x4*>(t + (long long)row * ldt + i0) = v;
       }
     }
     __syncthreads();
@@ -233,6 +289,7 @@ __global__ __launch_bounds__(256) void k_shrink_rows(const T* __restrict__ X, lo
     const Frag8<T> x = frag_load(xr + k);
 #pragma unroll
     for (int i = 0; i < SR_RANKS; ++i) a[i] = frag_load(ar[i] + k);
+    all_loads_first();
     step(x, a, k);
   }
   if (k < K) {
@@ -255,10 +312,6 @@ __global__ __launch_bounds__(256) void k_shrink_rows(const T* __restrict__ X, lo
 // ---- the projection with the low-rank part: out (M, Nn) = X (M, Kk) W^T (+ bias) + t Bt_a^T, tiles of BM x BN in LDS, rows of
 // 128 bytes along the reduction, 16-byte chunks XOR-ed with the row (conflict-free 16-byte reads).  Two LDS buffers and one
 // barrier a step: the step after next is on its way to registers while a step is computed.
-template <typename T> struct Lines { static constexpr int V = 16 / sizeof(T), KB = 128 / sizeof(T); };
-template <typename T> struct alignas(16) Line { T v[16 / sizeof(T)]; };
-template <typename T> struct alignas(sizeof(T)) LooseLine { T v[16 / sizeof(T)]; };     // the same at the alignment of one value
-
 __device__ __forceinline__ f32x16 mma32(uint4 a, uint4 b, f32x16 c, f16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
@@ -272,17 +325,37 @@ __device__ __forceinline__ f32x16 mma32(uint4 a, uint4 b, f32x16 c, float) {
   return c;
 }
 
-template <typename T> __device__ __forceinline__ uint4 line_load(const T* p) {
-  return __builtin_bit_cast(uint4, *reinterpret_cast<const LooseLine<T>*>(p));
-}
-// the first n values of a line (n <= 0: none), zero behind them
-template <typename T> __device__ __forceinline__ uint4 line_load(const T* p, int n) {
-  constexpr int V = Lines<T>::V;
-  if (n >= V) return line_load(p);
-  Line<T> o;
+// eight 32-bit values as a high and a low bf16 part
+__device__ __forceinline__ void split8(const float* v, bf16x8& hi, bf16x8& lo) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) o.v[j] = j < n ? p[j] : (T)0.f;
-  return __builtin_bit_cast(uint4, o);
+  for (int j = 0; j < 8; ++j) {
+    hi[j] = (bf16)v[j];
+    const float f = (float)hi[j];
+    lo[j] = (bf16)(fabsf(f) < INFINITY ? v[j] - f : 0.f);
+  }
+}
+// the low-rank term of one 32 x 32 block: b (outputs) times v (rows), over 2 V ranks
+__device__ __forceinline__ f32x16 mma_low(uint4 b, const float (&v)[8], f32x16 c, bf16) {
+  bf16x8 hi, lo;
+  split8(v, hi, lo);
+  const bf16x8 x = __builtin_bit_cast(bf16x8, b);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, lo, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, hi, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma_low(uint4 b, const float (&v)[8], f32x16 c, f16) {
+  bf16x8 hi, lo, bh, bl;
+  split8(v, hi, lo);
+  const f16x8 x = __builtin_bit_cast(f16x8, b);
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (float)x[j];
+  split8(f, bh, bl);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bh, lo, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bl, hi, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bh, hi, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma_low(uint4 b, const float (&v)[4], f32x16 c, float) {
+  return mma32(b, __builtin_bit_cast(uint4, f32x4{v[0], v[1], v[2], v[3]}), c, 0.f);
 }
 
 struct LowRank {
@@ -389,24 +462,18 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
             const int i = i0 + V * h;                 // at most ldt - 8 + V: a half that lies behind the rank reads the other's
             const bool in = i < lr.rank;
             f32x4 t4[V / 4];
-            Line<T> hi, lo;
+            float v[V];
 #pragma unroll
             for (int j = 0; j < V / 4; ++j) t4[j] = *reinterpret_cast<const f32x4*>(tr + (in ? i : i0) + 4 * j);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const float v = in ? t4[j / 4][j % 4] : 0.f;
-              hi.v[j] = (T)v;
-              const float f = (float)hi.v[j];
-              lo.v[j] = (T)(fabsf(f) < INFINITY ? v - f : 0.f);
-            }
+            for (int j = 0; j < V; ++j) v[j] = in ? t4[j / 4][j % 4] : 0.f;
 #pragma unroll
             for (int n = 0; n < NI; ++n) {
               const int col = n0 + (wn * NI + n) * 32 + l32;
               const T* bp = ba + (col < Nn ? col : Nn - 1) * lr.sn;
               uint4 bf = whole ? line_load(bp + (in ? i : i0)) : line_load(bp + i, lr.rank - i);
               if (!in) bf = uint4{0, 0, 0, 0};
-              add[n] = mma32(bf, __builtin_bit_cast(uint4, hi), add[n], T());
-              if (sizeof(T) == 2) add[n] = mma32(bf, __builtin_bit_cast(uint4, lo), add[n], T());
+              add[n] = mma_low(bf, v, add[n], T());
             }
           }
 #pragma unroll
@@ -494,7 +561,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
         for (int j = 0; j < 4; ++j) p.v[j] = (T)(acc[n][m][4 * j4 + j] + sb[wn * NI * 32 + col + j]);
         *reinterpret_cast<P*>(reinterpret_cast<T*>(mine + l32 * LD) + col) = p;
       }
-    __builtin_amdgcn_wave_barrier();
+    wave_sees_lds();
 #pragma unroll
     for (int i = 0; i < 32 * PER / 64; ++i) {
       const int r = i * (64 / PER) + lane / PER, u = lane % PER, col = cw + u * V;
@@ -512,135 +579,177 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
         }
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_sees_lds();
   }
 }
 
 // ---- few rows (M <= 64): the weights are read once, sixteen outputs a workgroup, its waves share the reduction
-constexpr int FEW_ROWS = 64, FEW_WAVES = 8, FEW_AHEAD = 4;
+constexpr int FEW_ROWS = 64, FEW_WAVES = 8;
 
 template <typename T, int MT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ W,
                                                                 long long ldw, int N, const T* __restrict__ bias, LowRank lr, Segs sg,
                                                                 T* __restrict__ out, long long ldo) {
-  __shared__ f32x4 red[FEW_WAVES][MT][64];
+  constexpr int U = strip_units<1, MT>();
+  __shared__ uint4 lds[FEW_WAVES * U];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, full = K >> 5;
-  f32x4 acc[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const T *wp = W + (n0 + l16 < N ? n0 + l16 : N - 1) * ldw + 8 * g, *xp[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) xp[m] = X + (16 * m + l16 < sg.M ? 16 * m + l16 : sg.M - 1) * ldx + 8 * g;
-  int s = w;
-  for (; s + FEW_WAVES * (FEW_AHEAD - 1) < full; s += FEW_WAVES * FEW_AHEAD) {
-    Frag8<T> a[FEW_AHEAD], x[FEW_AHEAD][MT];
-#pragma unroll
-    for (int u = 0; u < FEW_AHEAD; ++u) {
-      a[u] = frag_load(wp + 32 * (s + FEW_WAVES * u));
-#pragma unroll
-      for (int m = 0; m < MT; ++m) x[u][m] = frag_load(xp[m] + 32 * (s + FEW_WAVES * u));
-    }
-#pragma unroll
-    for (int u = 0; u < FEW_AHEAD; ++u)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m] = mma16(a[u], x[u][m], acc[m]);
-  }
-  for (; s < full; s += FEW_WAVES) {
-    const Frag8<T> a = frag_load(wp + 32 * s);
-    Frag8<T> x[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) x[m] = frag_load(xp[m] + 32 * s);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] = mma16(a, x[m], acc[m]);
-  }
-  if (K > 32 * full && w == full % FEW_WAVES) {
-    const int n = K - 32 * full - 8 * g;
-    const Frag8<T> a = frag_load(wp + 32 * full, n);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] = mma16(a, frag_load(xp[m] + 32 * full, n), acc[m]);
-  }
-#pragma unroll
-  for (int m = 0; m < MT; ++m) red[w][m][lane] = acc[m];
-  __syncthreads();
-  if (w >= MT) return;
-  f32x4 v = red[0][w][lane];
-#pragma unroll
-  for (int u = 1; u < FEW_WAVES; ++u) v += red[u][w][lane];
-  // lane: row 16 w + l16, outputs n0 + 4 g .. + 3
+  const int n0 = blockIdx.x * 16;
+  // wave w finishes rows 16 w .. 16 w + 15, lane: row 16 w + l16, outputs n0 + 4 g .. + 3.  Its adapter: how many requests start
+  // at or before the row, 64 of them looked at at a time by all lanes
   const int row = 16 * w + l16, col = n0 + 4 * g;
   int a = -1;
-  if (lr.t != nullptr && row < sg.M) {
-    int lo = 0, hi = sg.S;                             // last request that starts at or before the row
-    while (lo < hi) { const int mid = (lo + hi) >> 1; if (sg.row_start[mid] <= row) lo = mid + 1; else hi = mid; }
-    if (lo > 0) a = seg_span(sg, lo - 1, row, row + 1).a;
+  if (lr.t != nullptr && w < MT) {
+    int before = 0;
+    for (int s0 = 0; s0 < sg.S; s0 += 64) {
+      const int start = s0 + lane < sg.S ? sg.row_start[s0 + lane] : 0x7fffffff;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int n = __popcll(__ballot(start <= 16 * w + r));
+        before += l16 == r ? n : 0;
+      }
+    }
+    if (before > 0 && row < sg.M) a = seg_span(sg, before - 1, row, row + 1).a;
   }
+  f32x4 acc[MT][1];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+  strip_sum<T, 1, MT, FEW_WAVES, false>(acc, W + (long long)n0 * ldw, ldw, N - n0, X, ldx, sg.M, K, lds + w * U, w, lane, KeepArgs{}, KeepKey{}, 0);
+  f32x4* red = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) red[w * U + m * 64 + lane] = acc[m][0];
+  __syncthreads();
+  if (w >= MT || row >= sg.M) return;
+  f32x4 v = red[w * 64 + lane];
+#pragma unroll
+  for (int u = 1; u < FEW_WAVES; ++u) v += red[u * U + w * 64 + lane];
   if (a >= 0) {
     const T* b = static_cast<const T*>(lr.b) + (long long)a * lr.sa;
-    for (int i = 0; i < lr.rank; ++i) {
-      const float ti = lr.t[(long long)row * lr.ldt + i];
+    const float* tr = lr.t + (long long)row * lr.ldt;
+    if (lr.rank % 8 == 0) {
+      for (int i = 0; i < lr.rank; i += 8) {
+        const f32x4 t0 = *reinterpret_cast<const f32x4*>(tr + i), t1 = *reinterpret_cast<const f32x4*>(tr + i + 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < N) v[j] = fmaf(ti, (float)b[(col + j) * lr.sn + i], v[j]);
+        for (int j = 0; j < 4; ++j) {
+          const Frag8<T> f = frag_load(b + (col + j < N ? col + j : N - 1) * lr.sn + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j] = fmaf(t1[e], (float)f.v[e + 4], fmaf(t0[e], (float)f.v[e], v[j]));
+        }
+      }
+    } else {
+      for (int i = 0; i < lr.rank; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = fmaf(tr[i], (float)b[(col + j < N ? col + j : N - 1) * lr.sn + i], v[j]);
     }
   }
-  if (row < sg.M) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (col + j < N) out[row * ldo + col + j] = (T)(v[j] + (bias != nullptr ? (float)bias[col + j] : 0.f));
-  }
+  for (int j = 0; j < 4; ++j)
+    if (col + j < N) out[row * ldo + col + j] = (T)(v[j] + (bias != nullptr ? (float)bias[col + j] : 0.f));
 }
 
 // ---- sums over rows: G_a[p][i] = sum over the rows m of adapter a of X[m][p] t[m][i], 128 columns p and up to 64 ranks a
-// workgroup.  The reduction runs along the rows, so both operands are read as they lie: 16 x 16 x 4 fp32 products, lane (p, m).
-// The fp32 matrix rate is above what reading X needs up to a rank of 16 and keeps t exact.
-constexpr int OU_COLS = 128, OU_AHEAD = 4;
+// workgroup.  The reduction runs along the rows, while a row lies along its columns.  A lane loads eight columns of each of its
+// rows (whole lines), so what the matrix cores need -- consecutive rows of one column -- is in its own registers:
+//   fp32    four rows a wave and step, 16 x 16 x 4 products, column j of every lane at a time;
+//   16 bit  32 rows a wave and step (eight a lane), turned 8 x 8 in registers, 16 x 16 x 32 bf16 products with t split in two
+//           (an eighth of the matrix time of the fp32 products, which bounded ranks over 16).
+constexpr int OU_COLS = 128;
 
-// adds rows [lo, hi) to the sums of the four waves: wave w takes four rows of every sixteen
-template <typename T, int RT>
-__device__ __forceinline__ void outer_rows(f32x4 (&acc)[8][RT], const T* X, long long ldx, int P, const float* t, int rank, int ldt, int ib,
-                                           int p, int lo, int hi, int w, int lane, bool drop, const KeepArgs& ka, KeepKey key) {
-  const int l16 = lane & 15, g = lane >> 4;
-  int at[RT];                                          // ranks past the rank are read as the last one: not stored
+template <typename T, int RT> struct OuterSum {
+  const T* X;
+  const float* t;
+  const KeepArgs& ka;
+  KeepKey key;
+  long long ldx;
+  int P, p, ldt, g;
+  int at[RT];              // ranks past the rank are read as the last one: not stored
+  bool drop;
+  __device__ __forceinline__ OuterSum(const T* X_, long long ldx_, int P_, const float* t_, int ldt_, int ib, int p_, int lane, bool drop_,
+                                      const KeepArgs& ka_)
+      : X(X_), t(t_), ka(ka_), key(keep_key(ka_)), ldx(ldx_), P(P_), p(p_), ldt(ldt_), g(lane >> 4), drop(drop_) {
 #pragma unroll
-  for (int i = 0; i < RT; ++i) at[i] = ib + 16 * i + l16 < ldt ? ib + 16 * i + l16 : ldt - 1;
-  auto step = [&](Frag8<T> x, const float (&tv)[RT], int m) {
-    if (drop) {
-      uint32_t keep = keep8(ka, key, (uint64_t)m, (uint32_t)(p >> 3));
-      if (p & 7) keep = (keep | keep8(ka, key, (uint64_t)m, (uint32_t)(p >> 3) + 1) << 8) >> (p & 7);
-      frag_keep(x, keep);
+    for (int i = 0; i < RT; ++i) { const int r = ib + 16 * i + (lane & 15); at[i] = r < ldt ? r : ldt - 1; }
+  }
+  __device__ __forceinline__ void mask(Frag8<T>& x, int m) const {
+    uint32_t keep = keep8(ka, key, (uint64_t)m, (uint32_t)(p >> 3));
+    if (p & 7) keep = (keep | keep8(ka, key, (uint64_t)m, (uint32_t)(p >> 3) + 1) << 8) >> (p & 7);
+    frag_keep(x, keep);
+  }
+  // adds rows [lo, hi) to the sums of the four waves
+  __device__ __forceinline__ void rows(f32x4 (&acc)[8][RT], int lo, int hi, int w) const;
+  template <bool ALL> __device__ __forceinline__ void group(f32x4 (&acc)[8][RT], int m0, int hi) const;
+};
+
+__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma_outer(bf16x8 x, bf16x8 hi, bf16x8 lo, f32x4 c) { return mma16(x, hi, mma16(x, lo, c)); }
+__device__ __forceinline__ f32x4 mma_outer(f16x8 x, bf16x8 hi, bf16x8 lo, f32x4 c) {
+  float f[8];
+  bf16x8 xh, xl;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (float)x[j];
+  split8(f, xh, xl);
+  return mma16(xh, hi, mma16(xl, hi, mma16(xh, lo, c)));
+}
+
+// one step of a wave; ALL: every row lies before hi and a lane has its eight columns
+template <typename T, int RT>
+template <bool ALL>
+__device__ __forceinline__ void OuterSum<T, RT>::group(f32x4 (&acc)[8][RT], int m0, int hi) const {
+  constexpr int R = sizeof(T) == 2 ? 8 : 1;            // rows of a lane
+  Frag8<T> x[R];
+  float tv[RT][R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int m = m0 + R * g + r;
+    if (ALL) {
+      x[r] = frag_load(X + m * ldx + p);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) tv[i][r] = t[(long long)m * ldt + at[i]];
+    } else {
+      const bool in = m < hi;
+      x[r] = frag_load(X + (in ? m : m0) * ldx + p, in ? P - p : 0);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) tv[i][r] = in ? t[(long long)m * ldt + at[i]] : 0.f;
     }
+  }
+  if (sizeof(T) == 2) all_loads_first();
+  if (drop) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) mask(x[r], m0 + R * g + r);
+  }
+  if constexpr (sizeof(T) == 2) {
+    bf16x8 th[RT], tl[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) split8(tv[i], th[i], tl[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      decltype(x[0].v) col;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) col[r] = x[r].v[j];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) acc[j][i] = mma_outer(col, th[i], tl[i], acc[j][i]);
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[j], tv[i], acc[j][i], 0, 0, 0);
-  };
-  int m0 = lo + 4 * w;
+      for (int j = 0; j < 8; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[0].v[j], tv[i][0], acc[j][i], 0, 0, 0);
+  }
+}
+
+template <typename T, int RT>
+__device__ __forceinline__ void OuterSum<T, RT>::rows(f32x4 (&acc)[8][RT], int lo, int hi, int w) const {
+  constexpr int STEP = sizeof(T) == 2 ? 32 : 4;        // rows of a wave and step
+  int m0 = lo + STEP * w;
   if (P >= 8) {
-    for (; m0 + 16 * (OU_AHEAD - 1) + 4 <= hi; m0 += 16 * OU_AHEAD) {          // the loads of sixteen rows in flight
-      Frag8<T> x[OU_AHEAD];
-      float tv[OU_AHEAD][RT];
+    if constexpr (sizeof(T) == 4) {
+      for (; m0 + 12 * STEP + STEP <= hi; m0 += 16 * STEP) {                   // the loads of four steps in flight
 #pragma unroll
-      for (int u = 0; u < OU_AHEAD; ++u) {
-        const long long m = m0 + 16 * u + g;
-        x[u] = frag_load(X + m * ldx + p);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) tv[u][i] = t[m * ldt + at[i]];
+        for (int u = 0; u < 4; ++u) group<true>(acc, m0 + 4 * STEP * u, hi);
       }
-#pragma unroll
-      for (int u = 0; u < OU_AHEAD; ++u) step(x[u], tv[u], m0 + 16 * u + g);
     }
+    for (; m0 + STEP <= hi; m0 += 4 * STEP) group<true>(acc, m0, hi);
   }
-  for (; m0 < hi; m0 += 16) {
-    const int m = m0 + g;
-    const bool in = m < hi;
-    const T* xr = X + (long long)(in ? m : lo) * ldx + p;
-    const Frag8<T> x = frag_load(xr, in ? P - p : 0);
-    float tv[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) tv[i] = in ? t[(long long)m * ldt + at[i]] : 0.f;
-    step(x, tv, m);
-  }
+  for (; m0 < hi; m0 += 4 * STEP) group<false>(acc, m0, hi);
 }
 
 // first of the eight columns of a lane: the last lanes of a row share its last eight (they come to the same bits)
@@ -687,7 +796,6 @@ __device__ __forceinline__ void outer_run(const Outer& o, const Segs& sg, const 
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15;
   const int pb = blockIdx.x, run = blockIdx.y, chunks = (rank + 63) / 64;
   const int r0 = run * rows_per_run, r1 = sg.M - r0 < rows_per_run ? sg.M : r0 + rows_per_run;
-  const KeepKey key = keep_key(ka);
   int q = seg_find(sg, r0);
   for (q = q < 0 ? 0 : q; q < sg.S && sg.row_start[q] < r1; ++q) {
     const Span sp = seg_span(sg, q, r0, r1);
@@ -698,7 +806,8 @@ __device__ __forceinline__ void outer_run(const Outer& o, const Segs& sg, const 
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int i = 0; i < RT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      outer_rows<T, RT>(acc, static_cast<const T*>(o.X), o.ldx, o.P, o.t, rank, o.ldt, 64 * rc, outer_col(o.P, pb, l16), sp.lo, sp.hi, w, lane, o.drop != 0, ka, key);
+      OuterSum<T, RT>(static_cast<const T*>(o.X), o.ldx, o.P, o.t, o.ldt, 64 * rc, outer_col(o.P, pb, l16), lane, o.drop != 0, ka)
+          .rows(acc, sp.lo, sp.hi, w);
       f32x4* to = reinterpret_cast<f32x4*>(o.part) + part_at<RT>(o, run + q, pb, rc, chunks);
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
@@ -773,7 +882,6 @@ __global__ __launch_bounds__(256) void k_outer_direct(Outer oa, Outer ob, Segs s
   const int chunks = (rank + 63) / 64, a = blockIdx.y, pb = blockIdx.x / chunks, ib = 64 * (blockIdx.x % chunks);
   if (pb >= o.blocks) return;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15;
-  const KeepKey key = keep_key(ka);
   f32x4 acc[8][RT];
 #pragma unroll
   for (int j = 0; j < 8; ++j)
@@ -784,9 +892,8 @@ __global__ __launch_bounds__(256) void k_outer_direct(Outer oa, Outer ob, Segs s
     for (int e = 0; e < list.n; ++e) {
       const int q = list.q[e];
       const int lo = sg.row_start[q] > 0 ? sg.row_start[q] : 0, hi = sg.row_start[q + 1] < sg.M ? sg.row_start[q + 1] : sg.M;
-      const T* X = static_cast<const T*>(o.X);
-      const int p = outer_col(o.P, pb, l16);
-      outer_rows<T, RT>(acc, X, o.ldx, o.P, o.t, rank, o.ldt, ib, p, lo, hi, w, lane, o.drop != 0, ka, key);
+      OuterSum<T, RT>(static_cast<const T*>(o.X), o.ldx, o.P, o.t, o.ldt, ib, outer_col(o.P, pb, l16), lane, o.drop != 0, ka)
+          .rows(acc, lo, hi, w);
     }
   }
 #pragma unroll
@@ -800,19 +907,34 @@ __global__ __launch_bounds__(256) void k_outer_direct(Outer oa, Outer ob, Segs s
   }
 }
 
-// ---- transposes for the backward pass: out[z][c][r] = in[z][r][c] (rows x cols), out rows padded with zeros to ldo
-template <typename T>
-__global__ __launch_bounds__(256) void k_turn(const T* __restrict__ in, long long ldi, long long si, int rows, int cols,
-                                              T* __restrict__ out, long long ldo, long long so) {
+// ---- transposes for the backward pass, up to three in one launch: out[z][c][r] = in[z][r][c] (rows x cols), rows of out padded
+// with zeros to ldo
+struct Turn {
+  const void* in;
+  long long ldi, si;
+  int rows, cols;
+  void* out;
+  long long ldo, so;
+  int first, across, down; // first workgroup of the job, workgroups along the columns and the rows
+};
+struct Turns { Turn job[3]; int n; };
+
+template <typename T> __global__ __launch_bounds__(256) void k_turn(Turns all) {
   __shared__ T tile[64][66];
-  const T* i = in + blockIdx.z * si;
-  T* o = out + blockIdx.z * so;
-  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  int at = 0;
+  while (at + 1 < all.n && (int)blockIdx.x >= all.job[at + 1].first) ++at;
+  const Turn& jb = all.job[at];
+  const int id = blockIdx.x - jb.first, bx = id % jb.across, by = id / jb.across % jb.down, z = id / (jb.across * jb.down);
+  const T* i = static_cast<const T*>(jb.in) + z * jb.si;
+  T* o = static_cast<T*>(jb.out) + z * jb.so;
+  const int c0 = bx * 64, r0 = by * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll 4
   for (int j = ty; j < 64; j += 4)
-    tile[j][tx] = r0 + j < rows && c0 + tx < cols ? i[(r0 + j) * ldi + c0 + tx] : (T)0.f;
+    tile[j][tx] = r0 + j < jb.rows && c0 + tx < jb.cols ? i[(r0 + j) * jb.ldi + c0 + tx] : (T)0.f;
   __syncthreads();
+#pragma unroll 4
   for (int j = ty; j < 64; j += 4)
-    if (c0 + j < cols && r0 + tx < ldo) o[(c0 + j) * ldo + r0 + tx] = tile[tx][j];
+    if (c0 + j < jb.cols && r0 + tx < jb.ldo) o[(c0 + j) * jb.ldo + r0 + tx] = tile[tx][j];
 }
 
 // ---- host side
@@ -903,10 +1025,13 @@ int shrink(const hm_adapter_args& g, const T* X, long long ldx, int K, const T* 
     else hipLaunchKernelGGL((k_shrink_rows<T, false>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t, pad8(g.rank));
   } else {
     const dim3 grid((unsigned)((g.rows + SH_ROWS - 1) / SH_ROWS), (g.rank + SH_RANKS - 1) / SH_RANKS);
-#define HM_GO(RT, D) hipLaunchKernelGGL((k_shrink<T, RT, D>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t, pad8(g.rank))
-    if (g.rank <= 16) { if (drop) HM_GO(1, true); else HM_GO(1, false); }
-    else if (g.rank <= 32) { if (drop) HM_GO(2, true); else HM_GO(2, false); }
-    else { if (drop) HM_GO(4, true); else HM_GO(4, false); }
+#define HM_GO(RT, NW, D) hipLaunchKernelGGL((k_shrink<T, RT, NW, D>), grid, dim3(64 * NW), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t, pad8(g.rank))
+#define HM_GO_RT(RT) if (wide) { if (drop) HM_GO(RT, 8, true); else HM_GO(RT, 8, false); } else { if (drop) HM_GO(RT, 4, true); else HM_GO(RT, 4, false); }
+    const bool wide = K > 8 * Lines<T>::KB;            // more than eight lines: eight waves share them instead of four
+    if (g.rank <= 16) { HM_GO_RT(1) }
+    else if (g.rank <= 32) { HM_GO_RT(2) }
+    else { HM_GO_RT(4) }
+#undef HM_GO_RT
 #undef HM_GO
   }
   HM_CHECK_HIP(hipGetLastError());
@@ -952,11 +1077,11 @@ template <typename T> int forward(const hm_adapter_args& g, const KeepArgs& ka, 
   return project<T>(g, X, g.ld_x, g.k, W, g.ld_w, g.n, bias, lr, false, ka, y, ld_y, st);
 }
 
-template <typename T>
-int turn(const T* in, long long ldi, long long si, int rows, int cols, T* out, long long ldo, long long so, int count, hipStream_t st) {
-  hipLaunchKernelGGL((k_turn<T>), dim3((cols + 63) / 64, (unsigned)((ldo + 63) / 64), count), dim3(256), 0, st, in, ldi, si, rows, cols, out, ldo, so);
-  HM_CHECK_HIP(hipGetLastError());
-  return 0;
+void add_turn(Turns* all, int* blocks, const void* in, long long ldi, long long si, int rows, int cols, void* out, long long ldo,
+              long long so, int count) {
+  const Turn t = {in, ldi, si, rows, cols, out, ldo, so, *blocks, (cols + 63) / 64, (int)((ldo + 63) / 64)};
+  all->job[all->n++] = t;
+  *blocks += t.across * t.down * count;
 }
 
 template <typename T>
@@ -967,15 +1092,19 @@ int backward(const hm_adapter_args& g, const KeepArgs& ka, const void* d_dy, lon
   T *wt = reinterpret_cast<T*>(ws + p.wt), *bt = reinterpret_cast<T*>(ws + p.bt), *at = reinterpret_cast<T*>(ws + p.at);
   float* u = reinterpret_cast<float*>(ws + p.u);
   const bool any = g.adapters > 0 && g.segments > 0 && g.rows > 0;
-  int rc;
-  if (any && (d_dx != nullptr || d_da != nullptr)) {
-    if ((rc = turn<T>(static_cast<const T*>(g.d_b), g.rank, (long long)g.n * g.rank, g.n, g.rank, bt, p.npad, g.rank * p.npad, g.adapters, st))) return rc;
-    if ((rc = shrink<T>(g, dy, ld_dy, g.n, bt, p.npad, g.rank * p.npad, false, ka, u, st))) return rc;
-    // u carries s_a; the factor of the dropout joins where the mask does
+  const bool want_u = any && (d_dx != nullptr || d_da != nullptr), want_dx = d_dx != nullptr && g.rows > 0;
+  Turns turns = {};
+  int blocks = 0;
+  if (want_u) add_turn(&turns, &blocks, g.d_b, g.rank, (long long)g.n * g.rank, g.n, g.rank, bt, p.npad, g.rank * p.npad, g.adapters);
+  if (want_dx) add_turn(&turns, &blocks, W, g.ld_w, 0, g.n, g.k, wt, p.npad, 0, 1);
+  if (want_dx && any) add_turn(&turns, &blocks, g.d_a, g.k, (long long)g.rank * g.k, g.rank, g.k, at, p.rpad, g.k * p.rpad, g.adapters);
+  if (turns.n > 0) {
+    hipLaunchKernelGGL((k_turn<T>), dim3(blocks), dim3(256), 0, st, turns);
+    HM_CHECK_HIP(hipGetLastError());
   }
-  if (d_dx != nullptr && g.rows > 0) {
-    if ((rc = turn<T>(W, g.ld_w, 0, g.n, g.k, wt, p.npad, 0, 1, st))) return rc;
-    if (any && (rc = turn<T>(static_cast<const T*>(g.d_a), g.k, (long long)g.rank * g.k, g.rank, g.k, at, p.rpad, g.k * p.rpad, g.adapters, st))) return rc;
+  int rc;
+  if (want_u && (rc = shrink<T>(g, dy, ld_dy, g.n, bt, p.npad, g.rank * p.npad, false, ka, u, st))) return rc;
+  if (want_dx) {
     const LowRank lr = {any ? u : nullptr, at, g.k * p.rpad, p.rpad, g.rank, pad8(g.rank)};
     if ((rc = project<T>(g, dy, ld_dy, g.n, wt, p.npad, g.k, nullptr, lr, ka.threshold != 0, ka, static_cast<T*>(d_dx), ld_dx, st))) return rc;
   }
@@ -985,7 +1114,7 @@ int backward(const hm_adapter_args& g, const KeepArgs& ka, const void* d_dy, lon
                 d_da != nullptr ? (g.k + OU_COLS - 1) / OU_COLS : 0, ka.threshold != 0, ka.up};
     Outer ob = {dy, ld_dy, d_db != nullptr ? g.n : 0, d_t, pad8(g.rank), d_db, (long long)g.n * g.rank, g.rank, 1, reinterpret_cast<float*>(ws + p.pb),
                 d_db != nullptr ? (g.n + OU_COLS - 1) / OU_COLS : 0, 0, 1.f};
-    const int blocks = oa.blocks > ob.blocks ? oa.blocks : ob.blocks;
+    const int blocks = oa.blocks > ob.blocks ? oa.blocks : ob.blocks;   // column blocks
 #define HM_GO(RT)                                                                                                                    \
     if (p.direct) {                                                                                                                  \
       hipLaunchKernelGGL((k_outer_direct<T, RT>), dim3(blocks * p.chunks, g.adapters, 2), dim3(256), 0, st, oa, ob, sg, ka, g.rank); \

@@ -1,6 +1,7 @@
 """Thin torch-tensor wrappers over the C ABI (device pointers + current stream; no torch types cross the ABI)."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -108,9 +109,13 @@ def _check_draws(p, seed, tag, row0, device) -> tuple:
     return p, int(seed), word, int(tag), int(row0)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
-    """The device of a call's tensors as the current one, and its stream."""
-    return torch.cuda.device(device), torch.cuda.current_stream(device).cuda_stream
+    """The device of a call's tensors as the current one (left alone where it is), and its current stream."""
+    here = torch.cuda.current_device() == device.index
+    return _HERE if here else torch.cuda.device(device), torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _dropout_forward(x, relu, draws):
@@ -176,30 +181,27 @@ def _adapter_args(x, weight, bias, A, B, scale, row_start, adapter, draws) -> _l
 
 def _adapter_forward(x, weight, bias, A, B, scale, row_start, adapter, draws):
     args = _adapter_args(x, weight, bias, A, B, scale, row_start, adapter, draws)
-    n = weight.shape[0]
+    n, f32 = weight.shape[0], torch.float32
     y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    t = torch.empty(args.rows, (args.rank + 7) // 8 * 8, dtype=torch.float32, device=x.device)
+    t = torch.empty(args.rows, (args.rank + 7) // 8 * 8, dtype=f32, device=x.device)
     guard, stream = _on(x.device)
     with guard:
         _lib.check(_lib.lib().hm_adapter_linear(ctypes.byref(args), y.data_ptr(), n, t.data_ptr(), stream), "hm_adapter_linear")
-    return y, t
+    return y, t, args
 
 
 class _AdapterLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, A, B, weight, bias, scale, row_start, adapter, draws):
-        y, t = _adapter_forward(x, weight, bias, A, B, scale, row_start, adapter, draws)
-        p, seed, word, tag, row0 = draws
-        ctx.draws = (p, seed, tag, row0)
-        ctx.save_for_backward(x, A, B, weight, scale, row_start, adapter, t, word)
+        y, t, ctx.args = _adapter_forward(x, weight, bias, A, B, scale, row_start, adapter, draws)
+        ctx.save_for_backward(x, A, B, weight, scale, row_start, adapter, t, draws[2])
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, A, B, weight, scale, row_start, adapter, t, word = ctx.saved_tensors
-        p, seed, tag, row0 = ctx.draws
-        args = _adapter_args(x, weight, None, A, B, scale, row_start, adapter, (p, seed, word, tag, row0))
+        x, A, B, _, _, _, _, t, _ = ctx.saved_tensors        # ctx.args points into these: unchanged, or this line raises
+        args = ctx.args
         dy, _, _, ld = _rows_of_grad(dy)
         want_x, want_a, want_b = ctx.needs_input_grad[:3]
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
@@ -209,7 +211,7 @@ class _AdapterLinear(torch.autograd.Function):
         size = lib.hm_adapter_linear_backward_bytes(ctypes.byref(args))
         if size < 0:
             _lib.check(int(size), "hm_adapter_linear_backward_bytes")
-        ws = torch.empty(max(1, size), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         guard, stream = _on(x.device)
         with guard:
             _lib.check(lib.hm_adapter_linear_backward(ctypes.byref(args), dy.data_ptr(), ld, t.data_ptr(), _ptr(dx), x.shape[-1],
