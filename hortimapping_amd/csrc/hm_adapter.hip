@@ -365,6 +365,177 @@ struct LowRank {
   int rank, ldt;           // ldt: the rank rounded up to 8
 };
 
+// What a tile's rows m0 .. m1 - 1 belong to: the first request that may hold some of them, and whether it holds them all
+struct Owner { int q, a; bool whole; };
+template <typename Starts> __device__ __forceinline__ Owner owner_of(const Segs& sg, const Starts& of, int m0, int m1) {
+  Owner o = {of.find(m0), -1, false};
+  if (o.q < 0) o.q = 0;
+  if (o.q < sg.S) {
+    o.whole = of.start(o.q) <= m0 && of.start(o.q + 1) >= m1;
+    o.a = of.adapter(o.q);
+    if (o.a >= sg.n_adapters) o.a = -1;
+  }
+  return o;
+}
+// row_start and adapter where they lie
+struct InMemory {
+  const Segs& sg;
+  __device__ __forceinline__ int find(int row) const { return seg_find(sg, row); }
+  __device__ __forceinline__ int start(int q) const { return sg.row_start[q]; }
+  __device__ __forceinline__ int adapter(int q) const { return sg.adapter[q]; }
+};
+
+// adds the low-rank term to one wave's row of blocks: rows mb .. mb + 31, outputs nw ..
+template <typename T, int NI>
+__device__ __forceinline__ void low_rank(f32x16 (&sum)[NI], const LowRank& lr, const Segs& sg, const Owner& own, int Nn, int m1, int mb, int nw,
+                                         int lane) {
+  constexpr int V = Lines<T>::V;
+  const int l32 = lane & 31, h = lane >> 5, row = mb + l32;
+  const bool even = lr.rank % V == 0;                 // whole lines of B
+  // a half wave whose ranks lie behind the last reads the other half's and gets zeros
+  auto ranks = [&](const float* tr, int i0, float (&v)[V]) {
+    const int i = i0 + V * h;
+    const bool in = i < lr.rank;
+    f32x4 t4[V / 4];
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) t4[j] = *reinterpret_cast<const f32x4*>(tr + (in ? i : i0) + 4 * j);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = in ? t4[j / 4][j % 4] : 0.f;
+  };
+  auto outputs = [&](const T* ba, int n, int i0) {
+    const int i = i0 + V * h, col = nw + n * 32 + l32;
+    const bool in = i < lr.rank;
+    const T* bp = ba + (col < Nn ? col : Nn - 1) * lr.sn;
+    const uint4 b = even ? line_load(bp + (in ? i : i0)) : line_load(bp + i, lr.rank - i);
+    return in ? b : uint4{0, 0, 0, 0};
+  };
+  if (own.whole) {                                    // one request's: no selection
+    if (own.a < 0) return;
+    const T* ba = static_cast<const T*>(lr.b) + (long long)own.a * lr.sa;
+    const float* tr = lr.t + (long long)(row < m1 ? row : m1 - 1) * lr.ldt;
+#pragma unroll 1
+    for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
+      float v[V];
+      uint4 b[NI];
+      ranks(tr, i0, v);
+#pragma unroll
+      for (int n = 0; n < NI; ++n) b[n] = outputs(ba, n, i0);
+#pragma unroll
+      for (int n = 0; n < NI; ++n) sum[n] = mma_low(b[n], v, sum[n], T());
+    }
+    return;
+  }
+  const int r1 = mb + 32 < m1 ? mb + 32 : m1;
+#pragma unroll 1
+  for (int q = own.q; q < sg.S && sg.row_start[q] < r1; ++q) {
+    const Span sp = seg_span(sg, q, mb, r1);
+    if (sp.a < 0) continue;
+    const bool mine = row >= sp.lo && row < sp.hi;
+    const T* ba = static_cast<const T*>(lr.b) + (long long)sp.a * lr.sa;
+    const float* tr = lr.t + (long long)(mine ? row : sp.lo) * lr.ldt;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      f32x16 add = sum[n];
+#pragma unroll 1
+      for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
+        float v[V];
+        ranks(tr, i0, v);
+        add = mma_low(outputs(ba, n, i0), v, add, T());
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[n][j] = mine ? add[j] : sum[n][j];
+    }
+  }
+}
+
+// the low-rank term of one 32 x 32 block of dx with its mask and the factor of what the mask keeps
+template <typename T>
+__device__ __forceinline__ f32x16 masked_low_rank(const LowRank& lr, const Segs& sg, const KeepArgs& ka, KeepKey key, const Owner& own, int Nn, int m1,
+                                                  int mb, int nb, int lane) {
+  const int l32 = lane & 31, h = lane >> 5, cb = nb >> 3;
+  f32x16 add[1];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) add[0][j] = 0.f;
+  low_rank<T, 1>(add, lr, sg, own, Nn, m1, mb, nb, lane);
+  // lane h makes the draws of column blocks 2 h and 2 h + 1; its partner holds the other half of each block's columns
+  const uint64_t row = (uint64_t)(mb + l32);
+  const uint32_t k2 = keep8(ka, key, row, cb + 2 * h) | keep8(ka, key, row, cb + 2 * h + 1) << 8;
+  const uint32_t o2 = __shfl_xor(k2, 32);
+  const uint32_t k4 = h == 0 ? (k2 | o2 << 16) : (o2 | k2 << 16);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) add[0][j] = (k4 >> (8 * (j >> 2) + 4 * h + (j & 3))) & 1 ? add[0][j] * ka.up : 0.f;
+  return add[0];
+}
+
+// one 32 x 32 block of results: a lane holds four outputs of a row, its partner (lane ^ 32) the next four.  Of 16-bit results the
+// two exchange halves of a pair of groups, so that each stores eight neighbours: 16 bytes a lane, 32 of a row, either way
+template <typename T>
+__device__ __forceinline__ void store_block(const f32x16& sum, T* out, long long ldo, int m1, int Nn, int mb, int nb, int lane) {
+  constexpr int V = Lines<T>::V;
+  const int l32 = lane & 31, h = lane >> 5, row = mb + l32;
+  if (nb >= Nn) return;
+  T* o = out + (long long)row * ldo + nb;
+#pragma unroll
+  for (int p = 0; p < 32 / (2 * V); ++p) {
+    Line<T> x;
+    if constexpr (sizeof(T) == 2) {
+      typedef T Two __attribute__((ext_vector_type(2)));
+      uint32_t d[2][2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int at = 4 * (2 * p + e) + 2 * j;
+          d[e][j] = __builtin_bit_cast(uint32_t, Two{(T)sum[at], (T)sum[at + 1]});
+        }
+      uint4 q;
+      const auto lo = __builtin_amdgcn_permlane32_swap(d[0][0], d[1][0], false, false);
+      const auto hi = __builtin_amdgcn_permlane32_swap(d[0][1], d[1][1], false, false);
+      q.x = lo[0]; q.y = hi[0]; q.z = lo[1]; q.w = hi[1];
+      x = __builtin_bit_cast(Line<T>, q);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x.v[j] = sum[4 * p + j];
+    }
+    const int col = p * 2 * V + h * V;
+    if (row < m1) {
+      if (nb + col + V <= Nn) {
+        *reinterpret_cast<LooseLine<T>*>(o + col) = __builtin_bit_cast(LooseLine<T>, x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) if (nb + col + j < Nn) o[col + j] = x.v[j];
+      }
+    }
+  }
+}
+
+// the end of a wave's blocks (rows mw .., outputs nw ..): low-rank term (DROP: with the mask of x, in dx), bias, and out
+template <typename T, int NI, int MI, bool DROP>
+__device__ __forceinline__ void finish(const f32x16 (&acc)[NI][MI], const LowRank& lr, const Segs& sg, const KeepArgs& ka, const Owner& own, int Nn,
+                                       int m1, int mw, int nw, const float* sb, T* out, long long ldo, int lane) {
+  const int h = lane >> 5;
+  const KeepKey key = keep_key(ka);
+#pragma unroll
+  for (int m = 0; m < MI; ++m) {
+    const int mb = mw + m * 32;
+    f32x16 sum[NI];
+#pragma unroll
+    for (int n = 0; n < NI; ++n)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[n][j] = acc[n][m][j] + sb[n * 32 + 8 * (j >> 2) + 4 * h + (j & 3)];
+    if (lr.t != nullptr && mb < m1) {
+      if (!DROP) {
+        low_rank<T, NI>(sum, lr, sg, own, Nn, m1, mb, nw, lane);
+      } else {
+#pragma unroll
+        for (int n = 0; n < NI; ++n) sum[n] += masked_low_rank<T>(lr, sg, ka, key, own, Nn, m1, mb, nw + n * 32, lane);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NI; ++n) store_block<T>(sum[n], out, ldo, m1, Nn, mb, nw + n * 32, lane);
+  }
+}
+
 template <typename T, int BM, int BN, int WGM, int WGN, bool DROP>
 __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict__ X, long long ldx, int Kk, const T* __restrict__ W,
                                                             long long ldw, int Nn, const T* __restrict__ bias, LowRank lr, Segs sg,
@@ -438,70 +609,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[n][m][j] = 0.f;
 
-  if (lr.t != nullptr && busy) {
-    const T* b = static_cast<const T*>(lr.b);
-    const bool whole = lr.rank % V == 0;
-    int q = seg_find(sg, m0);
-    for (q = q < 0 ? 0 : q; q < sg.S && sg.row_start[q] < m1; ++q) {
-      const Span sp = seg_span(sg, q, m0, m1);
-      if (sp.a < 0) continue;
-      const T* ba = b + (long long)sp.a * lr.sa;
-#pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        const int row = m0 + (wm * MI + m) * 32 + l32;
-        const bool mine = row >= sp.lo && row < sp.hi;
-        if (__ballot(mine) != 0) {
-          const float* tr = lr.t + (long long)(mine ? row : sp.lo) * lr.ldt;
-          f32x16 add[NI];
-#pragma unroll
-          for (int n = 0; n < NI; ++n)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) add[n][j] = 0.f;
-#pragma unroll 1
-          for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
-            const int i = i0 + V * h;                 // at most ldt - 8 + V: a half that lies behind the rank reads the other's
-            const bool in = i < lr.rank;
-            f32x4 t4[V / 4];
-            float v[V];
-#pragma unroll
-            for (int j = 0; j < V / 4; ++j) t4[j] = *reinterpret_cast<const f32x4*>(tr + (in ? i : i0) + 4 * j);
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = in ? t4[j / 4][j % 4] : 0.f;
-#pragma unroll
-            for (int n = 0; n < NI; ++n) {
-              const int col = n0 + (wn * NI + n) * 32 + l32;
-              const T* bp = ba + (col < Nn ? col : Nn - 1) * lr.sn;
-              uint4 bf = whole ? line_load(bp + (in ? i : i0)) : line_load(bp + i, lr.rank - i);
-              if (!in) bf = uint4{0, 0, 0, 0};
-              add[n] = mma_low(bf, v, add[n], T());
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NI; ++n)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[n][m][j] = mine ? add[n][j] : acc[n][m][j];
-        }
-      }
-    }
-    if (DROP) {                                       // the mask of x on the low-rank part of dx
-      const KeepKey key = keep_key(ka);
-#pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        const int row = m0 + (wm * MI + m) * 32 + l32;
-#pragma unroll
-        for (int n = 0; n < NI; ++n) {
-          const int cb = (n0 + (wn * NI + n) * 32) >> 3;
-          // lane h makes the draws of column blocks 2 h and 2 h + 1; its partner holds the other half of each block's columns
-          const uint32_t k2 = keep8(ka, key, (uint64_t)row, cb + 2 * h) | keep8(ka, key, (uint64_t)row, cb + 2 * h + 1) << 8;
-          const uint32_t o2 = __shfl_xor(k2, 32);
-          const uint32_t k4 = h == 0 ? (k2 | o2 << 16) : (o2 | k2 << 16);
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[n][m][j] = (k4 >> (8 * (j >> 2) + 4 * h + (j & 3))) & 1 ? acc[n][m][j] * ka.up : 0.f;
-        }
-      }
-    }
-  }
+  Owner own = {0, -1, false};
+  if (lr.t != nullptr && busy) own = owner_of(sg, InMemory{sg}, m0, m1);
 
   const int rx = (wm * MI * 32 + l32) * 8, rw = (wn * NI * 32 + l32) * 8, sel = l32 & 7;    // rows of a block differ by 32: one XOR
   auto chunk = [&](int buf, int kk) {                 // 2 V values of the reduction
@@ -542,44 +651,311 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
   }
   if (!busy) return;
 
-  // results go out through the wave's own part of the LDS, 32 rows at a time, so that a row leaves in whole lines
-  constexpr int LD = NI * 32 * sizeof(T) / 16 + 1, PER = NI * 32 / V;       // 16-byte units of a row: with one of padding, and stored
-  static_assert(WGM * WGN * 32 * LD <= 2 * (BM + BN) * 8 && 64 % PER == 0, "");
-  uint4* mine = lds + w * 32 * LD;
-  const int cw = n0 + wn * NI * 32;
+  finish<T, NI, MI, DROP>(acc, lr, sg, ka, own, Nn, m1, m0 + wm * MI * 32, n0 + wn * NI * 32, sb + wn * NI * 32, out, ldo, lane);
+}
+
+// ---- the same for many tiles: 256 x 256, four waves of 128 x 128 (one a SIMD, with all its registers), one workgroup a CU that goes
+// from tile to tile.
+//
+// Bound by the matrix cores if everything else runs in their shadow: a wave has the fragments of the next chunk of the reduction on
+// their way from the LDS while it multiplies this one, and between the products writes its part of the next step into the other
+// buffer and sends for the step after that; one barrier a step, behind which the next step's first fragments are read.  128 x 128
+// outputs a wave need half an LDS byte for each that 128 x 64 need three quarters of.  Loads run on across tiles: a new tile's
+// first steps are under way while the last one is finished and stored.
+constexpr int WIDE = 256, LDS_REQUESTS = 256;
+
+// products whose sums stay where they are, in the accumulation registers.  Written out because all 256 of them hold sums: left to
+// itself the compiler lets a product write elsewhere than it read, has no register to write to, and moves sums through memory.
+// What it cannot see it does not wait for: two products on the same sum lie sixteen products apart, and sums_done() comes before
+// the sums are read.
+__device__ __forceinline__ void mma_here(f32x16& c, uint4 a, uint4 b, f16) {
+  asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(f32x4, a)), "v"(__builtin_bit_cast(f32x4, b)));
+}
+__device__ __forceinline__ void mma_here(f32x16& c, uint4 a, uint4 b, bf16) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(f32x4, a)), "v"(__builtin_bit_cast(f32x4, b)));
+}
+__device__ __forceinline__ void mma_here(f32x16& c, float a, float b) {
+  asm volatile("v_mfma_f32_32x32x2_f32 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+template <int NI, int MI> __device__ __forceinline__ void sums_done(f32x16 (&acc)[NI][MI]) {
+  asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[0][0]));     // more than the sixteen passes of the last product
 #pragma unroll
-  for (int m = 0; m < MI; ++m) {
-    const int rb = m0 + (wm * MI + m) * 32;
-    if (rb >= sg.M) break;
+  for (int n = 0; n < NI; ++n)
+#pragma unroll
+    for (int m = 0; m < MI; ++m) asm volatile("" : "+a"(acc[n][m]));
+}
+
+// the low-rank term of a wave's 128 x 128 outputs of a tile that is one request's, added where the sums are
+template <typename T>
+__device__ __forceinline__ void low_rank_here(f32x16 (&acc)[4][4], const LowRank& lr, const Owner& own, int Nn, int m1, int mw, int nw, int lane) {
+  constexpr int V = Lines<T>::V;
+  const int l32 = lane & 31, h = lane >> 5;
+  const bool even = lr.rank % V == 0;                 // whole lines of B
+  const T* ba = static_cast<const T*>(lr.b) + (long long)own.a * lr.sa;
+#pragma unroll 1
+  for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
+    const int i = i0 + V * h;
+    const bool in = i < lr.rank;                      // a half wave whose ranks lie behind the last reads the other half's and gets zeros
+    uint4 b[4];
+    f32x4 t4[4][V / 4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int col = nw + n * 32 + l32;
+      const T* bp = ba + (col < Nn ? col : Nn - 1) * lr.sn;
+      b[n] = even ? line_load(bp + (in ? i : i0)) : line_load(bp + i, lr.rank - i);
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int row = mw + m * 32 + l32;
+      const float* tr = lr.t + (long long)(row < m1 ? row : m1 - 1) * lr.ldt + (in ? i : i0);
+#pragma unroll
+      for (int j = 0; j < V / 4; ++j) t4[m][j] = *reinterpret_cast<const f32x4*>(tr + 4 * j);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) if (!in) b[n] = uint4{0, 0, 0, 0};
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 hi[4], lo[4], bh[4], bl[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = in ? t4[m][j / 4][j % 4] : 0.f;
+        split8(v, hi[m], lo[m]);
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if constexpr (__is_same(T, f16)) {
+          float f[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = (float)__builtin_bit_cast(f16x8, b[n])[j];
+          split8(f, bh[n], bl[n]);
+        } else {
+          bh[n] = __builtin_bit_cast(bf16x8, b[n]);
+        }
+      }
+#pragma unroll
+      for (int part = 0; part < (__is_same(T, f16) ? 3 : 2); ++part)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const int n = k >> 2, m = k & 3;
+          mma_here(acc[n][m], __builtin_bit_cast(uint4, part == 2 ? bl[n] : bh[n]), __builtin_bit_cast(uint4, part == 0 ? lo[m] : hi[m]), bf16());
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const int n = k >> 2, m = k & 3;
+          mma_here(acc[n][m], __builtin_bit_cast(f32x4, b[n])[j], in ? t4[m][0][j] : 0.f);
+        }
+    }
+  }
+}
+
+struct InLds {
+  const Segs& sg;
+  const int (*at)[LDS_REQUESTS];
+  int lane;
+  __device__ __forceinline__ int find(int row) const {
+    int n = 0;
+    for (int q = 0; q < sg.S; q += 64) n += __popcll(__ballot(q + lane < sg.S && at[0][q + lane] <= row));
+    return n - 1;
+  }
+  __device__ __forceinline__ int start(int q) const { return __builtin_amdgcn_readfirstlane(at[0][q]); }
+  __device__ __forceinline__ int adapter(int q) const { return __builtin_amdgcn_readfirstlane(at[1][q]); }
+};
+
+// a row's last n values (n = 1 .. V - 1), read as the 16 bytes that end with the row: moved down, zeros above; n <= 0: zeros
+template <typename T> __device__ __forceinline__ uint4 line_down(uint4 q, int n) {
+  constexpr int V = Lines<T>::V;
+  uint64_t lo = q.x | (uint64_t)q.y << 32, hi = q.z | (uint64_t)q.w << 32;
+  const int bits = (n >= V ? 0 : V - n) * 8 * (int)sizeof(T);
+  const bool far = bits >= 64;
+  const uint64_t a = far ? hi : lo, b = far ? 0 : hi;
+  const int r = bits & 63;
+  lo = a >> r | (r != 0 ? b << (64 - r) : 0);
+  hi = b >> r;
+  if (n <= 0) lo = hi = 0;
+  return uint4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+
+// `v`, which the compiler takes for a new value
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+template <typename T, bool DROP>
+__global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X, long long ldx, int Kk, const T* __restrict__ W, long long ldw,
+                                                         int Nn, const T* __restrict__ bias, LowRank lr, Segs sg, KeepArgs ka,
+                                                         T* __restrict__ out, long long ldo, int tiles_m, int tiles_n) {
+  constexpr int MI = 4, NI = 4, V = Lines<T>::V, KB = Lines<T>::KB;
+  __shared__ uint4 lds[2][2 * WIDE * 8];              // X lines, then W lines
+  __shared__ float sb[2][WIDE];                       // the bias, of this tile and the next
+  __shared__ int starts[2][LDS_REQUESTS];             // row_start, and the adapter of each request, where they are few
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
+  const int lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  // workgroups go to the eight XCDs in turn: each XCD takes a contiguous run of tiles, its 32 workgroups neighbours in it, in
+  // bands of eight tiles of rows (eight by four tiles at a time share what their L2 holds)
+  const int total = tiles_m * tiles_n, xcd = blockIdx.x & 7, each = total >> 3, extra = total & 7;
+  const int first = xcd * each + (xcd < extra ? xcd : extra), end = first + each + (xcd < extra ? 1 : 0);
+  auto place = [&](int tile, int& m0, int& n0) {
+    const int band = tile / (8 * tiles_n), in = tile - band * 8 * tiles_n;
+    const int high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+    m0 = (band * 8 + in % high) * WIDE;
+    n0 = in / high * WIDE;
+  };
+  const int full = Kk / KB, rest = Kk - full * KB, steps = full + (rest > 0);
+  const int rr = tid >> 3, c = tid & 7;
+  // the last step of a row that does not end with a line: the lane reads the 16 bytes that end with the row (or, where it has no
+  // value left, some of the step before) and moves them down when it writes them
+  const int left = rest - c * V;
+  const uint32_t tail_back = left >= V ? 0 : left > 0 ? (V - left) * (int)sizeof(T) : 128;
+  // where the loads are: tile, step, and what belongs to them (128 bytes before the step, for tail_back).  Rows past the end are
+  // read as the last one: a row touches its own results alone.  Behind the last tile its own steps are read again, and not used
+  int f_tile = first + (blockIdx.x >> 3), f_step = 0;
+  const char *fx, *fw;
+  uint32_t ox[8], ow[8], back = 128;
+  auto aim = [&]() {
+    int m0, n0;
+    place(f_tile, m0, n0);
+    fx = reinterpret_cast<const char*>(X + m0 * ldx) - 128;
+    fw = reinterpret_cast<const char*>(W + n0 * ldw) - 128;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = rr + 32 * j;
+      ox[j] = ((uint32_t)(m0 + r < sg.M ? r : sg.M - 1 - m0) * (uint32_t)ldx + c * V) * sizeof(T);
+      ow[j] = ((uint32_t)(n0 + r < Nn ? r : Nn - 1 - n0) * (uint32_t)ldw + c * V) * sizeof(T);
+    }
+  };
+  uint4 gl[16];                                       // eight lines of X, eight of W
+  auto fetch = [&](int j) {
+    gl[j] = j < 8 ? line_load(reinterpret_cast<const T*>(fx + (ox[j & 7] + back))) : line_load(reinterpret_cast<const T*>(fw + (ow[j & 7] + back)));
+  };
+  auto next = [&]() {
+    fx += 128;
+    fw += 128;
+    if (++f_step == steps) {
+      f_step = 0;
+      if (f_tile + 32 < end) f_tile += 32;
+      aim();
+    }
+    back = f_step < full ? 128 : 128 - tail_back;
+  };
+  const int to = rr * 8 + (c ^ (rr & 7));             // rows of a thread differ by 32: one XOR
+  auto stash = [&](int buf, int j, bool tail) {
+    // (made afresh from the thread's number: held over the loop it would be spilled, and a reload waits for every load under way)
+    if (tail) gl[j] = line_down<T>(gl[j], rest - (fresh(tid) & 7) * V);
+    lds[buf][(j < 8 ? 0 : WIDE * 8) + to + (j & 7) * 256] = gl[j];
+  };
+  int tile = f_tile;
+  if (tile >= end) return;
+  const bool cached = sg.S < LDS_REQUESTS;
+  if (cached && lr.t != nullptr) {
+    if (tid <= sg.S) starts[0][tid] = sg.row_start[tid];
+    if (tid < sg.S) starts[1][tid] = sg.adapter[tid];
+  }
+  aim();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) fetch(j);
+  next();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) stash(0, j, false);    // the host keeps full >= 1
+#pragma unroll
+  for (int j = 0; j < 16; ++j) fetch(j);
+  int s_step = f_step;                                // step that gl holds
+  next();
+  __syncthreads();
+  const int rx = (wm * 128 + l32) * 8, rw = WIDE * 8 + (wn * 128 + l32) * 8, sel = l32 & 7;
+  uint4 fr[2][8];                                     // fragments of this chunk and the next: four of W, four of X
+  auto read = [&](int buf, int kk, int set, int i) {
+    const int at = (2 * kk + h) ^ sel;
+    fr[set][i] = lds[buf][(i < 4 ? rw + i * 256 : rx + (i - 4) * 256) + at];
+  };
+  int buf = 0;
+  for (int turn = 0; tile < end; tile += 32, turn ^= 1) {
+    int m0, n0;
+    place(tile, m0, n0);
+    const int m1 = m0 + WIDE < sg.M ? m0 + WIDE : sg.M;
+    const int mw = m0 + wm * 128, nw = n0 + wn * 128;
+    const bool busy = nw < Nn;                        // a wave without outputs keeps step, and stores nothing
+    sb[turn][tid] = bias != nullptr && n0 + tid < Nn ? (float)bias[n0 + tid] : 0.f;
+    Owner own = {0, -1, false};
+    if (lr.t != nullptr) own = cached ? owner_of(sg, InLds{sg, starts, fresh(tid) & 63}, m0, m1) : owner_of(sg, InMemory{sg}, m0, m1);
+    f32x16 acc[NI][MI];
 #pragma unroll
     for (int n = 0; n < NI; ++n)
 #pragma unroll
-      for (int j4 = 0; j4 < 4; ++j4) {
-        const int col = n * 32 + 8 * j4 + 4 * h;
-        struct alignas(4 * sizeof(T)) P { T v[4]; } p;
+      for (int m = 0; m < MI; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p.v[j] = (T)(acc[n][m][4 * j4 + j] + sb[wn * NI * 32 + col + j]);
-        *reinterpret_cast<P*>(reinterpret_cast<T*>(mine + l32 * LD) + col) = p;
-      }
-    wave_sees_lds();
+        for (int j = 0; j < 16; ++j) acc[n][m][j] = 0.f;
+    const bool whole = !DROP && own.whole;
+    if (lr.t != nullptr && whole && own.a >= 0) low_rank_here<T>(acc, lr, own, Nn, m1, mw, nw, fresh(tid) & 63);
+    // (the last step of the tile before read these too; across its end they would take 32 registers)
 #pragma unroll
-    for (int i = 0; i < 32 * PER / 64; ++i) {
-      const int r = i * (64 / PER) + lane / PER, u = lane % PER, col = cw + u * V;
-      const Line<T> v = __builtin_bit_cast(Line<T>, mine[r * LD + u]);
-      T* o = out + (long long)(rb + r) * ldo + col;
-      if (rb + r < sg.M) {
-        if (col + V <= Nn) {
-          LooseLine<T> x;
+    for (int i = 0; i < 8; ++i) read(buf, 0, 0, i);
+    for (int s = 0; s < steps; ++s) {
+      const bool tail = s_step >= full;
 #pragma unroll
-          for (int j = 0; j < V; ++j) x.v[j] = v.v[j];
-          *reinterpret_cast<LooseLine<T>*>(o) = x;
-        } else {
+      for (int kk = 0; kk < 4; ++kk) {
+        const int now = kk & 1;
+        if (kk == 3) __syncthreads();                 // the next step lies in the LDS, and no fragment of the one before this is waited for
 #pragma unroll
-          for (int j = 0; j < V; ++j) if (col + j < Nn) o[j] = v.v[j];
+        for (int j = 0; j < (sizeof(T) == 2 ? 1 : 4); ++j) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (j == 0) {
+              if (kk < 3) read(buf, kk + 1, now ^ 1, i);
+              else read(buf ^ 1, 0, now ^ 1, i);
+              if (kk == 1 || kk == 2) {
+                stash(buf ^ 1, (kk - 1) * 8 + i, tail);
+                fetch((kk - 1) * 8 + i);
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int n = (2 * i + e) >> 2, m = (2 * i + e) & 3;
+              if constexpr (sizeof(T) == 2) {
+                mma_here(acc[n][m], fr[now][n], fr[now][4 + m], T());
+              } else {
+                mma_here(acc[n][m], __builtin_bit_cast(f32x4, fr[now][n])[j], __builtin_bit_cast(f32x4, fr[now][4 + m])[j]);
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
       }
+      s_step = f_step;
+      next();
+      buf ^= 1;
     }
-    wave_sees_lds();
+    sums_done(acc);
+    if (!busy) continue;
+    // block by block, in ONE place that reads the sums: wherever else they were read the compiler would keep a copy, in memory
+    const KeepKey key = keep_key(ka);
+#pragma unroll 1
+    for (int k = 0; k < NI * MI; ++k) {
+      const int mb = mw + (k & 3) * 32, nb = nw + (k >> 2) * 32, ln = fresh(tid) & 63;
+      if (mb >= m1 || nb >= Nn) continue;
+      f32x16 sum[1], add;
+      if (DROP && lr.t != nullptr) add = masked_low_rank<T>(lr, sg, ka, key, own, Nn, m1, mb, nb, ln);
+#define HM_BLOCK(U) case U: asm volatile("; block %0" ::"i"(U)); sum[0] = acc[U >> 2][U & 3]; break;     // (a branch, not 16 selections)
+      switch (k) {
+        HM_BLOCK(0) HM_BLOCK(1) HM_BLOCK(2) HM_BLOCK(3) HM_BLOCK(4) HM_BLOCK(5) HM_BLOCK(6) HM_BLOCK(7)
+        HM_BLOCK(8) HM_BLOCK(9) HM_BLOCK(10) HM_BLOCK(11) HM_BLOCK(12) HM_BLOCK(13) HM_BLOCK(14) HM_BLOCK(15)
+      }
+#undef HM_BLOCK
+      if (lr.t != nullptr && !whole) {                // several requests' rows, or a mask
+        if (DROP) sum[0] += add;
+        else low_rank<T, 1>(sum, lr, sg, own, Nn, m1, mb, nb, ln);
+      }
+      // a thread's outputs of a group of four: the bias of column nb + 8 (j / 4) + 4 h + j % 4
+      const float* b = sb[turn] + nb - n0 + (ln >> 5) * 4;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[0][j] += b[8 * (j >> 2) + (j & 3)];
+      store_block<T>(sum[0], out, ldo, m1, Nn, mb, nb, ln);
+    }
   }
 }
 
@@ -1046,8 +1422,13 @@ int project(const hm_adapter_args& g, const T* X, long long ldx, int Kk, const T
   hipLaunchKernelGGL((k_project<T, BM, BN, WGM, WGN, D>), dim3((unsigned)(((g.rows + BM - 1) / BM) * ((Nn + BN - 1) / BN))),         \
                      dim3(64 * WGM * WGN), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, (Nn + BN - 1) / BN)
   const long long big = ((g.rows + 255) / 256) * ((Nn + 255) / 256);
-  if (big >= 128) { if (drop) HM_GO(256, 256, 2, 4, true); else HM_GO(256, 256, 2, 4, false); }
-  else { if (drop) HM_GO(128, 128, 2, 2, true); else HM_GO(128, 128, 2, 2, false); }
+  if (big >= 128 && Kk >= Lines<T>::KB) {
+    const int tm = (int)((g.rows + WIDE - 1) / WIDE), tn = (Nn + WIDE - 1) / WIDE;
+    const dim3 grid(big < 256 ? (unsigned)big : 256);
+    if (drop) hipLaunchKernelGGL((k_project_wide<T, true>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, tm, tn);
+    else hipLaunchKernelGGL((k_project_wide<T, false>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, tm, tn);
+  } else { if (drop) HM_GO(128, 128, 2, 2, true); else HM_GO(128, 128, 2, 2, false);
+  }
 #undef HM_GO
   HM_CHECK_HIP(hipGetLastError());
   return 0;
