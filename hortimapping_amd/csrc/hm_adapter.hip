@@ -334,13 +334,15 @@ __device__ __forceinline__ void split8(const float* v, bf16x8& hi, bf16x8& lo) {
     lo[j] = (bf16)(fabsf(f) < INFINITY ? v[j] - f : 0.f);
   }
 }
-// the low-rank term of one 32 x 32 block: b (outputs) times v (rows), over 2 V ranks
+// the low-rank term of one 32 x 32 block: b (outputs) times v (rows), over 2 V ranks.  Written out for sums in ordinary registers: the
+// wide projection keeps its own in all accumulation registers, which the compiler would take for these.  The waits are those
+// between dependent products and before a sum is read (sixteen passes at most).
 __device__ __forceinline__ f32x16 mma_low(uint4 b, const float (&v)[8], f32x16 c, bf16) {
   bf16x8 hi, lo;
   split8(v, hi, lo);
-  const bf16x8 x = __builtin_bit_cast(bf16x8, b);
-  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, lo, c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, hi, c, 0, 0, 0);
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0\n\ts_nop 9\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %3, %0\n\ts_nop 15\n\ts_nop 3"
+               : "+v"(c) : "v"(__builtin_bit_cast(f32x4, b)), "v"(__builtin_bit_cast(f32x4, lo)), "v"(__builtin_bit_cast(f32x4, hi)));
+  return c;
 }
 __device__ __forceinline__ f32x16 mma_low(uint4 b, const float (&v)[8], f32x16 c, f16) {
   bf16x8 hi, lo, bh, bl;
@@ -350,12 +352,18 @@ __device__ __forceinline__ f32x16 mma_low(uint4 b, const float (&v)[8], f32x16 c
 #pragma unroll
   for (int j = 0; j < 8; ++j) f[j] = (float)x[j];
   split8(f, bh, bl);
-  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bh, lo, c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bl, hi, c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bh, hi, c, 0, 0, 0);
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %3, %0\n\ts_nop 9\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %4, %0\n\ts_nop 9\n\t"
+               "v_mfma_f32_32x32x16_bf16 %0, %1, %4, %0\n\ts_nop 15\n\ts_nop 3"
+               : "+v"(c) : "v"(__builtin_bit_cast(f32x4, bh)), "v"(__builtin_bit_cast(f32x4, bl)), "v"(__builtin_bit_cast(f32x4, lo)),
+                 "v"(__builtin_bit_cast(f32x4, hi)));
+  return c;
 }
 __device__ __forceinline__ f32x16 mma_low(uint4 b, const float (&v)[4], f32x16 c, float) {
-  return mma32(b, __builtin_bit_cast(uint4, f32x4{v[0], v[1], v[2], v[3]}), c, 0.f);
+  const f32x4 x = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 %0, %1, %2, %0\n\ts_nop 15\n\ts_nop 3" : "+v"(c) : "v"(x[j]), "v"(v[j]));
+  return c;
 }
 
 struct LowRank {
@@ -467,45 +475,32 @@ __device__ __forceinline__ f32x16 masked_low_rank(const LowRank& lr, const Segs&
   return add[0];
 }
 
-// one 32 x 32 block of results: a lane holds four outputs of a row, its partner (lane ^ 32) the next four.  Of 16-bit results the
-// two exchange halves of a pair of groups, so that each stores eight neighbours: 16 bytes a lane, 32 of a row, either way
-template <typename T>
-__device__ __forceinline__ void store_block(const f32x16& sum, T* out, long long ldo, int m1, int Nn, int mb, int nb, int lane) {
+// 16 bytes of results of a 32 x 32 block: outputs 2 V q + V h .. of a lane's row.  A lane holds four outputs of a row and its partner
+// (lane ^ 32) the next four; of 16-bit results the two exchange halves of a pair of groups
+template <typename T> __device__ __forceinline__ uint4 line_of(const f32x16& sum, int q) {
+  if constexpr (sizeof(T) == 2) {
+    typedef T Two __attribute__((ext_vector_type(2)));
+    uint32_t d[2][2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) d[e][j] = __builtin_bit_cast(uint32_t, Two{(T)sum[8 * q + 4 * e + 2 * j], (T)sum[8 * q + 4 * e + 2 * j + 1]});
+    const auto lo = __builtin_amdgcn_permlane32_swap(d[0][0], d[1][0], false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap(d[0][1], d[1][1], false, false);
+    return uint4{lo[0], hi[0], lo[1], hi[1]};
+  } else {
+    return __builtin_bit_cast(uint4, f32x4{sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]});
+  }
+}
+// the first n of 16 bytes of results (n <= 0: none)
+template <typename T> __device__ __forceinline__ void store_line(T* o, uint4 v, int n) {
   constexpr int V = Lines<T>::V;
-  const int l32 = lane & 31, h = lane >> 5, row = mb + l32;
-  if (nb >= Nn) return;
-  T* o = out + (long long)row * ldo + nb;
+  if (n >= V) {
+    *reinterpret_cast<LooseLine<T>*>(o) = __builtin_bit_cast(LooseLine<T>, v);
+  } else {
+    const Line<T> x = __builtin_bit_cast(Line<T>, v);
 #pragma unroll
-  for (int p = 0; p < 32 / (2 * V); ++p) {
-    Line<T> x;
-    if constexpr (sizeof(T) == 2) {
-      typedef T Two __attribute__((ext_vector_type(2)));
-      uint32_t d[2][2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int at = 4 * (2 * p + e) + 2 * j;
-          d[e][j] = __builtin_bit_cast(uint32_t, Two{(T)sum[at], (T)sum[at + 1]});
-        }
-      uint4 q;
-      const auto lo = __builtin_amdgcn_permlane32_swap(d[0][0], d[1][0], false, false);
-      const auto hi = __builtin_amdgcn_permlane32_swap(d[0][1], d[1][1], false, false);
-      q.x = lo[0]; q.y = hi[0]; q.z = lo[1]; q.w = hi[1];
-      x = __builtin_bit_cast(Line<T>, q);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x.v[j] = sum[4 * p + j];
-    }
-    const int col = p * 2 * V + h * V;
-    if (row < m1) {
-      if (nb + col + V <= Nn) {
-        *reinterpret_cast<LooseLine<T>*>(o + col) = __builtin_bit_cast(LooseLine<T>, x);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) if (nb + col + j < Nn) o[col + j] = x.v[j];
-      }
-    }
+    for (int j = 0; j < V; ++j) if (j < n) o[j] = x.v[j];
   }
 }
 
@@ -524,15 +519,23 @@ __device__ __forceinline__ void finish(const f32x16 (&acc)[NI][MI], const LowRan
 #pragma unroll
       for (int j = 0; j < 16; ++j) sum[n][j] = acc[n][m][j] + sb[n * 32 + 8 * (j >> 2) + 4 * h + (j & 3)];
     if (lr.t != nullptr && mb < m1) {
+      const Owner o = own.whole ? own : owner_of(sg, InMemory{sg}, mb, mb + 32 < m1 ? mb + 32 : m1);
       if (!DROP) {
-        low_rank<T, NI>(sum, lr, sg, own, Nn, m1, mb, nw, lane);
+        low_rank<T, NI>(sum, lr, sg, o, Nn, m1, mb, nw, lane);
       } else {
 #pragma unroll
-        for (int n = 0; n < NI; ++n) sum[n] += masked_low_rank<T>(lr, sg, ka, key, own, Nn, m1, mb, nw + n * 32, lane);
+        for (int n = 0; n < NI; ++n) sum[n] += masked_low_rank<T>(lr, sg, ka, key, o, Nn, m1, mb, nw + n * 32, lane);
       }
     }
+    const int row = mb + (lane & 31);
 #pragma unroll
-    for (int n = 0; n < NI; ++n) store_block<T>(sum[n], out, ldo, m1, Nn, mb, nw + n * 32, lane);
+    for (int n = 0; n < NI; ++n)
+#pragma unroll
+      for (int q = 0; q < 16 / Lines<T>::V; ++q) {
+        const int col = nw + n * 32 + (2 * q + h) * Lines<T>::V;
+        const uint4 v = line_of<T>(sum[n], q);
+        if (row < m1) store_line<T>(out + (long long)row * ldo + col, v, Nn - col);
+      }
   }
 }
 
@@ -664,40 +667,72 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict_
 // first steps are under way while the last one is finished and stored.
 constexpr int WIDE = 256, LDS_REQUESTS = 256;
 
-// products whose sums stay where they are, in the accumulation registers.  Written out because all 256 of them hold sums: left to
-// itself the compiler lets a product write elsewhere than it read, has no register to write to, and moves sums through memory.
-// What it cannot see it does not wait for: two products on the same sum lie sixteen products apart, and sums_done() comes before
-// the sums are read.
-__device__ __forceinline__ void mma_here(f32x16& c, uint4 a, uint4 b, f16) {
-  asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(f32x4, a)), "v"(__builtin_bit_cast(f32x4, b)));
-}
-__device__ __forceinline__ void mma_here(f32x16& c, uint4 a, uint4 b, bf16) {
-  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(f32x4, a)), "v"(__builtin_bit_cast(f32x4, b)));
-}
-__device__ __forceinline__ void mma_here(f32x16& c, float a, float b) {
-  asm volatile("v_mfma_f32_32x32x2_f32 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-}
-template <int NI, int MI> __device__ __forceinline__ void sums_done(f32x16 (&acc)[NI][MI]) {
-  asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[0][0]));     // more than the sixteen passes of the last product
+// The sums of the wide projection, by the names of their registers: block (n, m) of a wave is a[16 (4 n + m)] .. + 15, all 256
+// accumulation registers.  The compiler is not asked to place them: as variables they are copied wherever two paths meet, there
+// is no register left to copy through, and sums travel through memory (measured: 13 us a tile instead of 3).  It has no other use
+// for these registers, since what it keeps fits the 256 others.  What it cannot see it does not wait for: two products on the
+// same sum lie at least two products apart (a product passes its sum on to the next by itself), and sums_done() comes before the
+// sums are read.
+#define HM_ALL_SUMS \
+  "a0", "a1", "a2", "a3", "a4", "a5", "a6", "a7", "a8", "a9", "a10", "a11", "a12", "a13", "a14", "a15", "a16", "a17", "a18", \
+  "a19", "a20", "a21", "a22", "a23", "a24", "a25", "a26", "a27", "a28", "a29", "a30", "a31", "a32", "a33", "a34", "a35", "a36", \
+  "a37", "a38", "a39", "a40", "a41", "a42", "a43", "a44", "a45", "a46", "a47", "a48", "a49", "a50", "a51", "a52", "a53", "a54", \
+  "a55", "a56", "a57", "a58", "a59", "a60", "a61", "a62", "a63", "a64", "a65", "a66", "a67", "a68", "a69", "a70", "a71", "a72", \
+  "a73", "a74", "a75", "a76", "a77", "a78", "a79", "a80", "a81", "a82", "a83", "a84", "a85", "a86", "a87", "a88", "a89", "a90", \
+  "a91", "a92", "a93", "a94", "a95", "a96", "a97", "a98", "a99", "a100", "a101", "a102", "a103", "a104", "a105", "a106", "a107", \
+  "a108", "a109", "a110", "a111", "a112", "a113", "a114", "a115", "a116", "a117", "a118", "a119", "a120", "a121", "a122", "a123", \
+  "a124", "a125", "a126", "a127", "a128", "a129", "a130", "a131", "a132", "a133", "a134", "a135", "a136", "a137", "a138", "a139", \
+  "a140", "a141", "a142", "a143", "a144", "a145", "a146", "a147", "a148", "a149", "a150", "a151", "a152", "a153", "a154", "a155", \
+  "a156", "a157", "a158", "a159", "a160", "a161", "a162", "a163", "a164", "a165", "a166", "a167", "a168", "a169", "a170", "a171", \
+  "a172", "a173", "a174", "a175", "a176", "a177", "a178", "a179", "a180", "a181", "a182", "a183", "a184", "a185", "a186", "a187", \
+  "a188", "a189", "a190", "a191", "a192", "a193", "a194", "a195", "a196", "a197", "a198", "a199", "a200", "a201", "a202", "a203", \
+  "a204", "a205", "a206", "a207", "a208", "a209", "a210", "a211", "a212", "a213", "a214", "a215", "a216", "a217", "a218", "a219", \
+  "a220", "a221", "a222", "a223", "a224", "a225", "a226", "a227", "a228", "a229", "a230", "a231", "a232", "a233", "a234", "a235", \
+  "a236", "a237", "a238", "a239", "a240", "a241", "a242", "a243", "a244", "a245", "a246", "a247", "a248", "a249", "a250", "a251", \
+  "a252", "a253", "a254", "a255"
+__device__ __forceinline__ void sums_clear() {
+  asm volatile("" ::: HM_ALL_SUMS);
 #pragma unroll
-  for (int n = 0; n < NI; ++n)
+  for (int i = 0; i < 256; ++i) asm volatile("v_accvgpr_write_b32 a[%0], 0" ::"i"(i));
+  asm volatile("s_nop 7");
+}
+__device__ __forceinline__ void sums_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }   // more than the sixteen passes of the last product
+__device__ __forceinline__ void sums_used() { asm volatile("" ::: HM_ALL_SUMS); }
+__device__ __forceinline__ f32x16 sums_of(int n, int m) {
+  f32x16 v;
 #pragma unroll
-    for (int m = 0; m < MI; ++m) asm volatile("" : "+a"(acc[n][m]));
+  for (int j = 0; j < 16; ++j) {
+    float x;
+    asm volatile("v_accvgpr_read_b32 %0, a[%1]" : "=v"(x) : "i"(16 * (4 * n + m) + j));
+    v[j] = x;
+  }
+  return v;
+}
+__device__ __forceinline__ void mma_sums(int n, int m, uint4 a, uint4 b, f16) {
+  asm volatile("v_mfma_f32_32x32x16_f16 a[%2:%3], %0, %1, a[%2:%3]" ::"v"(__builtin_bit_cast(f32x4, a)), "v"(__builtin_bit_cast(f32x4, b)),
+               "i"(16 * (4 * n + m)), "i"(16 * (4 * n + m) + 15));
+}
+__device__ __forceinline__ void mma_sums(int n, int m, uint4 a, uint4 b, bf16) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 a[%2:%3], %0, %1, a[%2:%3]" ::"v"(__builtin_bit_cast(f32x4, a)), "v"(__builtin_bit_cast(f32x4, b)),
+               "i"(16 * (4 * n + m)), "i"(16 * (4 * n + m) + 15));
+}
+__device__ __forceinline__ void mma_sums(int n, int m, float a, float b) {
+  asm volatile("v_mfma_f32_32x32x2_f32 a[%2:%3], %0, %1, a[%2:%3]" ::"v"(a), "v"(b), "i"(16 * (4 * n + m)), "i"(16 * (4 * n + m) + 15));
 }
 
-// the low-rank term of a wave's 128 x 128 outputs of a tile that is one request's, added where the sums are
-template <typename T>
-__device__ __forceinline__ void low_rank_here(f32x16 (&acc)[4][4], const LowRank& lr, const Owner& own, int Nn, int m1, int mw, int nw, int lane) {
-  constexpr int V = Lines<T>::V;
+// the low-rank term of row blocks FIRST .. LAST - 1 of a wave's 128 x 128 outputs, which belong to adapter a, added where the sums are
+template <typename T, int FIRST, int LAST>
+__device__ __forceinline__ void low_rank_here(const LowRank& lr, int a, int Nn, int m1, int mw, int nw, int lane) {
+  constexpr int V = Lines<T>::V, MB = LAST - FIRST;
   const int l32 = lane & 31, h = lane >> 5;
   const bool even = lr.rank % V == 0;                 // whole lines of B
-  const T* ba = static_cast<const T*>(lr.b) + (long long)own.a * lr.sa;
+  const T* ba = static_cast<const T*>(lr.b) + (long long)a * lr.sa;
 #pragma unroll 1
   for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
     const int i = i0 + V * h;
     const bool in = i < lr.rank;                      // a half wave whose ranks lie behind the last reads the other half's and gets zeros
     uint4 b[4];
-    f32x4 t4[4][V / 4];
+    f32x4 t4[MB][V / 4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const int col = nw + n * 32 + l32;
@@ -705,52 +740,59 @@ __device__ __forceinline__ void low_rank_here(f32x16 (&acc)[4][4], const LowRank
       b[n] = even ? line_load(bp + (in ? i : i0)) : line_load(bp + i, lr.rank - i);
     }
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int row = mw + m * 32 + l32;
+    for (int m = 0; m < MB; ++m) {
+      const int row = mw + (FIRST + m) * 32 + l32;
       const float* tr = lr.t + (long long)(row < m1 ? row : m1 - 1) * lr.ldt + (in ? i : i0);
 #pragma unroll
       for (int j = 0; j < V / 4; ++j) t4[m][j] = *reinterpret_cast<const f32x4*>(tr + 4 * j);
     }
 #pragma unroll
     for (int n = 0; n < 4; ++n) if (!in) b[n] = uint4{0, 0, 0, 0};
+    // (two products on the same sum lie at least two products apart)
     if constexpr (sizeof(T) == 2) {
-      bf16x8 hi[4], lo[4], bh[4], bl[4];
+      bf16x8 hi[MB], lo[MB];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
+      for (int m = 0; m < MB; ++m) {
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = in ? t4[m][j / 4][j % 4] : 0.f;
         split8(v, hi[m], lo[m]);
       }
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        if constexpr (__is_same(T, f16)) {
-          float f[8];
+      for (int n2 = 0; n2 < 4; n2 += 2) {
+        bf16x8 bh[2], bl[2];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = (float)__builtin_bit_cast(f16x8, b[n])[j];
-          split8(f, bh[n], bl[n]);
-        } else {
-          bh[n] = __builtin_bit_cast(bf16x8, b[n]);
+        for (int n = 0; n < 2; ++n) {
+          if constexpr (__is_same(T, f16)) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = (float)__builtin_bit_cast(f16x8, b[n2 + n])[j];
+            split8(f, bh[n], bl[n]);
+          } else {
+            bh[n] = __builtin_bit_cast(bf16x8, b[n2 + n]);
+          }
         }
+#pragma unroll
+        for (int part = 0; part < (__is_same(T, f16) ? 3 : 2); ++part)
+#pragma unroll
+          for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              mma_sums(n2 + n, FIRST + m, __builtin_bit_cast(uint4, part == 2 ? bl[n] : bh[n]), __builtin_bit_cast(uint4, part == 0 ? lo[m] : hi[m]), bf16());
+        __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int part = 0; part < (__is_same(T, f16) ? 3 : 2); ++part)
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const int n = k >> 2, m = k & 3;
-          mma_here(acc[n][m], __builtin_bit_cast(uint4, part == 2 ? bl[n] : bh[n]), __builtin_bit_cast(uint4, part == 0 ? lo[m] : hi[m]), bf16());
-        }
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const int n = k >> 2, m = k & 3;
-          mma_here(acc[n][m], __builtin_bit_cast(f32x4, b[n])[j], in ? t4[m][0][j] : 0.f);
-        }
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) mma_sums(n, FIRST + m, __builtin_bit_cast(f32x4, b[n])[j], in ? t4[m][0][j] : 0.f);
     }
   }
 }
+
+template <int N> struct Number { static constexpr int value = N; };
 
 struct InLds {
   const Segs& sg;
@@ -791,6 +833,7 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
                                                          T* __restrict__ out, long long ldo, int tiles_m, int tiles_n) {
   constexpr int MI = 4, NI = 4, V = Lines<T>::V, KB = Lines<T>::KB;
   __shared__ uint4 lds[2][2 * WIDE * 8];              // X lines, then W lines
+  __shared__ uint4 stage[4][256];                     // 32 lines of results a wave
   __shared__ float sb[2][WIDE];                       // the bias, of this tile and the next
   __shared__ int starts[2][LDS_REQUESTS];             // row_start, and the adapter of each request, where they are few
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
@@ -836,6 +879,7 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
     fx += 128;
     fw += 128;
     if (++f_step == steps) {
+      asm volatile("; another tile");                 // keeps this a branch: its 140 instructions would be run at every step
       f_step = 0;
       if (f_tile + 32 < end) f_tile += 32;
       aim();
@@ -843,9 +887,7 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
     back = f_step < full ? 128 : 128 - tail_back;
   };
   const int to = rr * 8 + (c ^ (rr & 7));             // rows of a thread differ by 32: one XOR
-  auto stash = [&](int buf, int j, bool tail) {
-    // (made afresh from the thread's number: held over the loop it would be spilled, and a reload waits for every load under way)
-    if (tail) gl[j] = line_down<T>(gl[j], rest - (fresh(tid) & 7) * V);
+  auto stash = [&](int buf, int j) {
     lds[buf][(j < 8 ? 0 : WIDE * 8) + to + (j & 7) * 256] = gl[j];
   };
   int tile = f_tile;
@@ -855,12 +897,18 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
     if (tid <= sg.S) starts[0][tid] = sg.row_start[tid];
     if (tid < sg.S) starts[1][tid] = sg.adapter[tid];
   }
+  auto bias_of = [&](int of, int half) {
+    int m0, n0;
+    place(of, m0, n0);
+    sb[half][tid] = bias != nullptr && n0 + tid < Nn ? (float)bias[n0 + tid] : 0.f;
+  };
+  bias_of(tile, 0);
   aim();
 #pragma unroll
   for (int j = 0; j < 16; ++j) fetch(j);
   next();
 #pragma unroll
-  for (int j = 0; j < 16; ++j) stash(0, j, false);    // the host keeps full >= 1
+  for (int j = 0; j < 16; ++j) stash(0, j);           // the host keeps full >= 1
 #pragma unroll
   for (int j = 0; j < 16; ++j) fetch(j);
   int s_step = f_step;                                // step that gl holds
@@ -879,23 +927,20 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
     const int m1 = m0 + WIDE < sg.M ? m0 + WIDE : sg.M;
     const int mw = m0 + wm * 128, nw = n0 + wn * 128;
     const bool busy = nw < Nn;                        // a wave without outputs keeps step, and stores nothing
-    sb[turn][tid] = bias != nullptr && n0 + tid < Nn ? (float)bias[n0 + tid] : 0.f;
+    auto owner = [&](int r0, int r1, int ln) { return cached ? owner_of(sg, InLds{sg, starts, ln}, r0, r1) : owner_of(sg, InMemory{sg}, r0, r1); };
     Owner own = {0, -1, false};
-    if (lr.t != nullptr) own = cached ? owner_of(sg, InLds{sg, starts, fresh(tid) & 63}, m0, m1) : owner_of(sg, InMemory{sg}, m0, m1);
-    f32x16 acc[NI][MI];
-#pragma unroll
-    for (int n = 0; n < NI; ++n)
-#pragma unroll
-      for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) acc[n][m][j] = 0.f;
-    const bool whole = !DROP && own.whole;
-    if (lr.t != nullptr && whole && own.a >= 0) low_rank_here<T>(acc, lr, own, Nn, m1, mw, nw, fresh(tid) & 63);
+    if (lr.t != nullptr) own = owner(m0, m1, fresh(tid) & 63);
+    sums_clear();
+    if (tile + 32 < end) bias_of(tile + 32, turn ^ 1);
     // (the last step of the tile before read these too; across its end they would take 32 registers)
 #pragma unroll
     for (int i = 0; i < 8; ++i) read(buf, 0, 0, i);
     for (int s = 0; s < steps; ++s) {
-      const bool tail = s_step >= full;
+      if (s_step >= full) {
+        const int n = rest - (fresh(tid) & 7) * V;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) gl[j] = line_down<T>(gl[j], n);
+      }
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         const int now = kk & 1;
@@ -908,7 +953,7 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
               if (kk < 3) read(buf, kk + 1, now ^ 1, i);
               else read(buf ^ 1, 0, now ^ 1, i);
               if (kk == 1 || kk == 2) {
-                stash(buf ^ 1, (kk - 1) * 8 + i, tail);
+                stash(buf ^ 1, (kk - 1) * 8 + i);
                 fetch((kk - 1) * 8 + i);
               }
             }
@@ -917,9 +962,9 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
             for (int e = 0; e < 2; ++e) {
               const int n = (2 * i + e) >> 2, m = (2 * i + e) & 3;
               if constexpr (sizeof(T) == 2) {
-                mma_here(acc[n][m], fr[now][n], fr[now][4 + m], T());
+                mma_sums(n, m, fr[now][n], fr[now][4 + m], T());
               } else {
-                mma_here(acc[n][m], __builtin_bit_cast(f32x4, fr[now][n])[j], __builtin_bit_cast(f32x4, fr[now][4 + m])[j]);
+                mma_sums(n, m, __builtin_bit_cast(f32x4, fr[now][n])[j], __builtin_bit_cast(f32x4, fr[now][4 + m])[j]);
               }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -930,32 +975,98 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
       next();
       buf ^= 1;
     }
-    sums_done(acc);
+    // the low-rank term comes after the main loop: before it, its loads would stand in line behind the stores of the tile before
+    // row blocks of 32 that lie in one request get their low-rank term here; bit m of `open`: block m does not
+    unsigned open = 0;
+    if (lr.t != nullptr) {
+      const int ln = fresh(tid) & 63;
+      if (DROP || !busy) {
+        open = 15;
+      } else if (own.whole) {
+        if (own.a >= 0) {
+          if constexpr (__is_same(T, f16)) {          // (its weights take two parts: half the rows at a time fit the registers)
+            low_rank_here<T, 0, 2>(lr, own.a, Nn, m1, mw, nw, ln);
+            low_rank_here<T, 2, 4>(lr, own.a, Nn, m1, mw, nw, ln);
+          } else {
+            low_rank_here<T, 0, 4>(lr, own.a, Nn, m1, mw, nw, ln);
+          }
+        }
+      } else {
+        auto block = [&](auto of) {
+          constexpr int M = decltype(of)::value;
+          const int r0 = mw + M * 32, r1 = r0 + 32 < m1 ? r0 + 32 : m1;
+          if (r0 >= m1) return;
+          const Owner o = owner(r0, r1, ln);
+          if (!o.whole) open |= 1u << M;
+          else if (o.a >= 0) low_rank_here<T, M, M + 1>(lr, o.a, Nn, m1, mw, nw, ln);
+        };
+        block(Number<0>()); block(Number<1>()); block(Number<2>()); block(Number<3>());
+      }
+    }
+    sums_done();
     if (!busy) continue;
-    // block by block, in ONE place that reads the sums: wherever else they were read the compiler would keep a copy, in memory
+    // 32 rows of 128 bytes at a time (two blocks of 16-bit results, one of fp32), through the wave's own part of the LDS: in the
+    // layout of the products a row's results leave in pieces of 32 bytes, which the memory path takes four times as long for
+    constexpr int PAIR = sizeof(T) == 2 ? 2 : 1;
     const KeepKey key = keep_key(ka);
 #pragma unroll 1
-    for (int k = 0; k < NI * MI; ++k) {
-      const int mb = mw + (k & 3) * 32, nb = nw + (k >> 2) * 32, ln = fresh(tid) & 63;
+    for (int k = 0; k < NI * MI; k += PAIR) {         // block k: outputs k % 4, rows k / 4
+      const int mb = mw + (k >> 2) * 32, nb = nw + (k & 3) * 32, ln = fresh(tid) & 63, l32 = ln & 31, h = ln >> 5;
       if (mb >= m1 || nb >= Nn) continue;
-      f32x16 sum[1], add;
-      if (DROP && lr.t != nullptr) add = masked_low_rank<T>(lr, sg, ka, key, own, Nn, m1, mb, nb, ln);
-#define HM_BLOCK(U) case U: asm volatile("; block %0" ::"i"(U)); sum[0] = acc[U >> 2][U & 3]; break;     // (a branch, not 16 selections)
-      switch (k) {
-        HM_BLOCK(0) HM_BLOCK(1) HM_BLOCK(2) HM_BLOCK(3) HM_BLOCK(4) HM_BLOCK(5) HM_BLOCK(6) HM_BLOCK(7)
-        HM_BLOCK(8) HM_BLOCK(9) HM_BLOCK(10) HM_BLOCK(11) HM_BLOCK(12) HM_BLOCK(13) HM_BLOCK(14) HM_BLOCK(15)
+      f32x16 sum[PAIR];
+#define HM_BLOCK(U)                                                       \
+      case U:                                                             \
+        sum[0] = sums_of(U & 3, U >> 2);                                  \
+        if constexpr (PAIR == 2) sum[PAIR - 1] = sums_of((U + 1) & 3, U >> 2); \
+        break;
+      if constexpr (PAIR == 2) {
+        switch (k) { HM_BLOCK(0) HM_BLOCK(2) HM_BLOCK(4) HM_BLOCK(6) HM_BLOCK(8) HM_BLOCK(10) HM_BLOCK(12) HM_BLOCK(14) }
+      } else {
+        switch (k) {
+          HM_BLOCK(0) HM_BLOCK(1) HM_BLOCK(2) HM_BLOCK(3) HM_BLOCK(4) HM_BLOCK(5) HM_BLOCK(6) HM_BLOCK(7)
+          HM_BLOCK(8) HM_BLOCK(9) HM_BLOCK(10) HM_BLOCK(11) HM_BLOCK(12) HM_BLOCK(13) HM_BLOCK(14) HM_BLOCK(15)
+        }
       }
 #undef HM_BLOCK
-      if (lr.t != nullptr && !whole) {                // several requests' rows, or a mask
-        if (DROP) sum[0] += add;
-        else low_rank<T, 1>(sum, lr, sg, own, Nn, m1, mb, nb, ln);
-      }
-      // a thread's outputs of a group of four: the bias of column nb + 8 (j / 4) + 4 h + j % 4
-      const float* b = sb[turn] + nb - n0 + (ln >> 5) * 4;
+      if (bias != nullptr) {                          // a lane's outputs are nb + 32 e + 8 (j / 4) + 4 h + j % 4
+        const float* b = sb[turn] + nb - n0 + 4 * h;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum[0][j] += b[8 * (j >> 2) + (j & 3)];
-      store_block<T>(sum[0], out, ldo, m1, Nn, mb, nb, ln);
+        for (int e = 0; e < PAIR; ++e)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum[e][j] += b[e * 32 + 8 * (j >> 2) + (j & 3)];
+      }
+      if (DROP ? lr.t != nullptr : open >> (k >> 2) & 1) {       // a mask, or several requests' rows
+        const Owner o = own.whole ? own : owner(mb, mb + 32 < m1 ? mb + 32 : m1, ln);
+#pragma unroll
+        for (int e = 0; e < PAIR; ++e) {
+          if (nb + e * 32 >= Nn) break;
+          if (DROP) {
+            sum[e] += masked_low_rank<T>(lr, sg, ka, key, o, Nn, m1, mb, nb + e * 32, ln);
+          } else {
+            f32x16 one[1] = {sum[e]};
+            low_rank<T, 1>(one, lr, sg, o, Nn, m1, mb, nb + e * 32, ln);
+            sum[e] = one[0];
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < PAIR; ++e)
+#pragma unroll
+        for (int q = 0; q < 4 / PAIR; ++q) stage[w][l32 * 8 + ((e * 4 + 2 * q + h) ^ (l32 & 7))] = line_of<T>(sum[e], q);
+      wave_sees_lds();
+      uint4 line[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { const int r = i * 8 + (ln >> 3); line[i] = stage[w][r * 8 + ((ln & 7) ^ (r & 7))]; }
+      const int col = nb + (ln & 7) * V;
+      T* o = out + (long long)(mb + (ln >> 3)) * ldo + col;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (mb + i * 8 + (ln >> 3) < m1) store_line<T>(o, line[i], Nn - col);
+        o += 8 * ldo;
+      }
+      wave_sees_lds();
     }
+    sums_used();
   }
 }
 
