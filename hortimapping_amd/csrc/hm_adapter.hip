@@ -949,25 +949,25 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
         for (int j = 0; j < (sizeof(T) == 2 ? 1 : 4); ++j) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (j == 0) {
-              if (kk < 3) read(buf, kk + 1, now ^ 1, i);
-              else read(buf ^ 1, 0, now ^ 1, i);
-              if (kk == 1 || kk == 2) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // at most two memory instructions between two products: more take longer to send than a product lasts
+              if (j == 0 && e == 0) {
+                if (kk < 3) read(buf, kk + 1, now ^ 1, i);
+                else read(buf ^ 1, 0, now ^ 1, i);
+              } else if (j == 0 && (kk == 1 || kk == 2)) {
                 stash(buf ^ 1, (kk - 1) * 8 + i);
                 fetch((kk - 1) * 8 + i);
               }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
+              __builtin_amdgcn_sched_barrier(0);
               const int n = (2 * i + e) >> 2, m = (2 * i + e) & 3;
               if constexpr (sizeof(T) == 2) {
                 mma_sums(n, m, fr[now][n], fr[now][4 + m], T());
               } else {
                 mma_sums(n, m, __builtin_bit_cast(f32x4, fr[now][n])[j], __builtin_bit_cast(f32x4, fr[now][4 + m])[j]);
               }
+              __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
