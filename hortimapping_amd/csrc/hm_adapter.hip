@@ -1070,8 +1070,9 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
   }
 }
 
-// ---- few rows (M <= 64): the weights are read once, sixteen outputs a workgroup, its waves share the reduction
-constexpr int FEW_ROWS = 64, FEW_WAVES = 8;
+// ---- few rows: the weights are read once for each 64 rows, sixteen outputs a workgroup, its waves share the reduction
+// (up to 256 rows: 45 us of 256 rows x 4096 x 4096 against 60 of the tiles of 64, 29 against 59 of 128 rows)
+constexpr int FEW_ROWS = 256, FEW_WAVES = 8;
 
 template <typename T, int MT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restrict__ X, long long ldx, int K, const T* __restrict__ W,
@@ -1081,9 +1082,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restr
   __shared__ uint4 lds[FEW_WAVES * U];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16;
-  // wave w finishes rows 16 w .. 16 w + 15, lane: row 16 w + l16, outputs n0 + 4 g .. + 3.  Its adapter: how many requests start
+  // wave w finishes rows m0 + 16 w .. m0 + 16 w + 15, lane: row m0 + 16 w + l16, outputs n0 + 4 g .. + 3.  Its adapter: how many requests start
   // at or before the row, 64 of them looked at at a time by all lanes
-  const int row = 16 * w + l16, col = n0 + 4 * g;
+  const int m0 = blockIdx.y * 64, row = m0 + 16 * w + l16, col = n0 + 4 * g;
   int a = -1;
   if (lr.t != nullptr && w < MT) {
     int before = 0;
@@ -1091,7 +1092,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restr
       const int start = s0 + lane < sg.S ? sg.row_start[s0 + lane] : 0x7fffffff;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int n = __popcll(__ballot(start <= 16 * w + r));
+        const int n = __popcll(__ballot(start <= m0 + 16 * w + r));
         before += l16 == r ? n : 0;
       }
     }
@@ -1100,7 +1101,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restr
   f32x4 acc[MT][1];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-  strip_sum<T, 1, MT, FEW_WAVES, false>(acc, W + (long long)n0 * ldw, ldw, N - n0, X, ldx, sg.M, K, lds + w * U, w, lane, KeepArgs{}, KeepKey{}, 0);
+  strip_sum<T, 1, MT, FEW_WAVES, false>(acc, W + (long long)n0 * ldw, ldw, N - n0, X + (long long)m0 * ldx, ldx, sg.M - m0, K, lds + w * U, w, lane, KeepArgs{}, KeepKey{}, 0);
   f32x4* red = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
   for (int m = 0; m < MT; ++m) red[w * U + m * 64 + lane] = acc[m][0];
@@ -1525,6 +1526,33 @@ int shrink(const hm_adapter_args& g, const T* X, long long ldx, int K, const T* 
   return 0;
 }
 
+// Outputs a side of a workgroup's tile: 256 (k_project_wide: whole rounds of one workgroup a CU count, the last one is as long as the
+// others), 128 (two a CU) or 64 (five).  By the time that rounds of each took on an MI355X, in us, with s steps of 128 bytes along the
+// reduction (rank 16):
+//   16 bits  wide 14 + 1.67 s a round of 256 tiles, 128: 4.7 + 1.29 s a round of 512; 64 where those of 128 would not fill the CUs once
+//            (512 x 4096 x 4096: 49 against 60) or half of each would lie beside the outputs
+//   fp32     wide 38 + 6.8 s a round, 64: 2.97 s a round of 1280 (128 takes as long from 2048 rows of 512 on, twice as long below)
+// e.g. 131072 x 512 x 512 bf16 wide 117, 128: 149, 64: 174; 52000 rows 76, 62, 69; 8192 x 4096 x 4096 256, 378, 616.
+int pick_tile(long long rows, int n, int k, int size) {
+  auto tiles = [&](int t) { return ((rows + t - 1) / t) * ((n + t - 1) / t); };
+  const int line = 128 / size;
+  const double s = (k + line - 1) / line, rounds = (double)((tiles(256) + 255) / 256);
+  double wide, other;
+  int small;
+  if (size == 2) {
+    wide = rounds * (14 + 1.67 * s);
+    const double r = tiles(128) / 512.0;
+    other = (r < 1 ? 1 : r) * (4.7 + 1.29 * s) + 2;
+    small = tiles(128) < 256 || n <= 64 ? 64 : 128;
+  } else {
+    wide = rounds * (38 + 6.8 * s);
+    const double r = tiles(64) / 1280.0;
+    other = (r < 1 ? 1 : r) * 2.97 * s + 5;
+    small = 64;
+  }
+  return k >= line && tiles(256) >= 64 && wide < other ? 256 : small;
+}
+
 template <typename T>
 int project(const hm_adapter_args& g, const T* X, long long ldx, int Kk, const T* W, long long ldw, int Nn, const T* bias,
             const LowRank& lr, bool drop, const KeepArgs& ka, T* out, long long ldo, hipStream_t st) {
@@ -1532,13 +1560,16 @@ int project(const hm_adapter_args& g, const T* X, long long ldx, int Kk, const T
 #define HM_GO(BM, BN, WGM, WGN, D)                                                                                                   \
   hipLaunchKernelGGL((k_project<T, BM, BN, WGM, WGN, D>), dim3((unsigned)(((g.rows + BM - 1) / BM) * ((Nn + BN - 1) / BN))),         \
                      dim3(64 * WGM * WGN), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, (Nn + BN - 1) / BN)
-  const long long big = ((g.rows + 255) / 256) * ((Nn + 255) / 256);
-  if (big >= 128 && Kk >= Lines<T>::KB) {
+  const int tile = pick_tile(g.rows, Nn, Kk, sizeof(T));
+  if (tile == 256) {
     const int tm = (int)((g.rows + WIDE - 1) / WIDE), tn = (Nn + WIDE - 1) / WIDE;
-    const dim3 grid(big < 256 ? (unsigned)big : 256);
+    const dim3 grid((long long)tm * tn < 256 ? tm * tn : 256);
     if (drop) hipLaunchKernelGGL((k_project_wide<T, true>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, tm, tn);
     else hipLaunchKernelGGL((k_project_wide<T, false>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, tm, tn);
-  } else { if (drop) HM_GO(128, 128, 2, 2, true); else HM_GO(128, 128, 2, 2, false);
+  } else if (tile == 128) {
+    if constexpr (sizeof(T) == 2) { if (drop) HM_GO(128, 128, 2, 2, true); else HM_GO(128, 128, 2, 2, false); }
+  } else {
+    if (drop) HM_GO(64, 64, 2, 2, true); else HM_GO(64, 64, 2, 2, false);
   }
 #undef HM_GO
   HM_CHECK_HIP(hipGetLastError());
@@ -1556,7 +1587,7 @@ template <typename T> int forward(const hm_adapter_args& g, const KeepArgs& ka, 
   }
   const LowRank lr = {any ? d_t : nullptr, g.d_b, (long long)g.n * g.rank, g.rank, g.rank, pad8(g.rank)};
   if (g.rows <= FEW_ROWS) {
-    const dim3 grid((g.n + 15) / 16);
+    const dim3 grid((g.n + 15) / 16, (unsigned)((g.rows + 63) / 64));
     const Segs sg = segs_of(g);
 #define HM_GO(MT) hipLaunchKernelGGL((k_project_few<T, MT>), grid, dim3(64 * FEW_WAVES), 0, st, X, g.ld_x, g.k, W, g.ld_w, g.n, bias, lr, sg, y, ld_y)
     if (g.rows <= 16) HM_GO(1);
