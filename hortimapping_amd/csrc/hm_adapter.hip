@@ -394,9 +394,10 @@ struct InMemory {
 };
 
 // adds the low-rank term to one wave's row of blocks: rows mb .. mb + 31, outputs nw ..
-template <typename T, int NI>
-__device__ __forceinline__ void low_rank(f32x16 (&sum)[NI], const LowRank& lr, const Segs& sg, const Owner& own, int Nn, int m1, int mb, int nw,
-                                         int lane) {
+// (`between` is run behind the first loads and before what waits for them)
+template <typename T, int NI, typename Starts, typename Between>
+__device__ __forceinline__ void low_rank(f32x16 (&sum)[NI], const LowRank& lr, const Segs& sg, const Starts& of, const Owner& own, int Nn, int m1,
+                                         int mb, int nw, int lane, Between&& between) {
   constexpr int V = Lines<T>::V;
   const int l32 = lane & 31, h = lane >> 5, row = mb + l32;
   const bool even = lr.rank % V == 0;                 // whole lines of B
@@ -418,7 +419,7 @@ __device__ __forceinline__ void low_rank(f32x16 (&sum)[NI], const LowRank& lr, c
     return in ? b : uint4{0, 0, 0, 0};
   };
   if (own.whole) {                                    // one request's: no selection
-    if (own.a < 0) return;
+    if (own.a < 0) { between(); return; }
     const T* ba = static_cast<const T*>(lr.b) + (long long)own.a * lr.sa;
     const float* tr = lr.t + (long long)(row < m1 ? row : m1 - 1) * lr.ldt;
 #pragma unroll 1
@@ -428,51 +429,68 @@ __device__ __forceinline__ void low_rank(f32x16 (&sum)[NI], const LowRank& lr, c
       ranks(tr, i0, v);
 #pragma unroll
       for (int n = 0; n < NI; ++n) b[n] = outputs(ba, n, i0);
+      if (i0 == 0) { all_loads_first(); between(); }
 #pragma unroll
       for (int n = 0; n < NI; ++n) sum[n] = mma_low(b[n], v, sum[n], T());
     }
     return;
   }
+  between();
   const int r1 = mb + 32 < m1 ? mb + 32 : m1;
 #pragma unroll 1
-  for (int q = own.q; q < sg.S && sg.row_start[q] < r1; ++q) {
-    const Span sp = seg_span(sg, q, mb, r1);
-    if (sp.a < 0) continue;
-    const bool mine = row >= sp.lo && row < sp.hi;
-    const T* ba = static_cast<const T*>(lr.b) + (long long)sp.a * lr.sa;
-    const float* tr = lr.t + (long long)(mine ? row : sp.lo) * lr.ldt;
+  for (int q = own.q; q < sg.S; ++q) {
+    const int s0 = of.start(q), s1 = of.start(q + 1), a = of.adapter(q);
+    if (s0 >= r1) break;
+    if (a < 0 || a >= sg.n_adapters || s1 <= mb || s1 <= s0) continue;
+    const bool mine = row >= s0 && row < s1 && row < r1;
+    const T* ba = static_cast<const T*>(lr.b) + (long long)a * lr.sa;
+    const float* tr = lr.t + (long long)(mine ? row : s0 > mb ? s0 : mb) * lr.ldt;
+    f32x16 add[NI];
 #pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      f32x16 add = sum[n];
+    for (int n = 0; n < NI; ++n) add[n] = sum[n];
 #pragma unroll 1
-      for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
-        float v[V];
-        ranks(tr, i0, v);
-        add = mma_low(outputs(ba, n, i0), v, add, T());
-      }
+    for (int i0 = 0; i0 < lr.rank; i0 += 2 * V) {
+      float v[V];
+      uint4 b[NI];
+      ranks(tr, i0, v);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum[n][j] = mine ? add[j] : sum[n][j];
+      for (int n = 0; n < NI; ++n) b[n] = outputs(ba, n, i0);
+#pragma unroll
+      for (int n = 0; n < NI; ++n) add[n] = mma_low(b[n], v, add[n], T());
     }
+#pragma unroll
+    for (int n = 0; n < NI; ++n)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[n][j] = mine ? add[n][j] : sum[n][j];
   }
 }
 
-// the low-rank term of one 32 x 32 block of dx with its mask and the factor of what the mask keeps
-template <typename T>
-__device__ __forceinline__ f32x16 masked_low_rank(const LowRank& lr, const Segs& sg, const KeepArgs& ka, KeepKey key, const Owner& own, int Nn, int m1,
-                                                  int mb, int nb, int lane) {
-  const int l32 = lane & 31, h = lane >> 5, cb = nb >> 3;
-  f32x16 add[1];
+// the low-rank term of a row of blocks of dx, with the mask of x and the factor of what it keeps, added
+template <typename T, int NI, typename Starts>
+__device__ __forceinline__ void masked_low_rank(f32x16 (&sum)[NI], const LowRank& lr, const Segs& sg, const Starts& of, const KeepArgs& ka, KeepKey key,
+                                                const Owner& own, int Nn, int m1, int mb, int nb, int lane) {
+  const int l32 = lane & 31, h = lane >> 5;
+  f32x16 add[NI];
+  uint32_t keep[NI];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) add[0][j] = 0.f;
-  low_rank<T, 1>(add, lr, sg, own, Nn, m1, mb, nb, lane);
-  // lane h makes the draws of column blocks 2 h and 2 h + 1; its partner holds the other half of each block's columns
-  const uint64_t row = (uint64_t)(mb + l32);
-  const uint32_t k2 = keep8(ka, key, row, cb + 2 * h) | keep8(ka, key, row, cb + 2 * h + 1) << 8;
-  const uint32_t o2 = __shfl_xor(k2, 32);
-  const uint32_t k4 = h == 0 ? (k2 | o2 << 16) : (o2 | k2 << 16);
+  for (int n = 0; n < NI; ++n)
 #pragma unroll
-  for (int j = 0; j < 16; ++j) add[0][j] = (k4 >> (8 * (j >> 2) + 4 * h + (j & 3))) & 1 ? add[0][j] * ka.up : 0.f;
-  return add[0];
+    for (int j = 0; j < 16; ++j) add[n][j] = 0.f;
+  low_rank<T, NI>(add, lr, sg, of, own, Nn, m1, mb, nb, lane, [&]() {
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      // lane h makes the draws of column blocks 2 h and 2 h + 1; its partner holds the other half of each block's columns
+      const uint64_t row = (uint64_t)(mb + l32);
+      const int cb = (nb >> 3) + 4 * n;
+      const uint32_t k2 = keep8(ka, key, row, cb + 2 * h) | keep8(ka, key, row, cb + 2 * h + 1) << 8;
+      const uint32_t o2 = __shfl_xor(k2, 32);
+      keep[n] = h == 0 ? (k2 | o2 << 16) : (o2 | k2 << 16);
+    }
+  });
+#pragma unroll
+  for (int n = 0; n < NI; ++n)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum[n][j] += (keep[n] >> (8 * (j >> 2) + 4 * h + (j & 3))) & 1 ? add[n][j] * ka.up : 0.f;
 }
 
 // 16 bytes of results of a 32 x 32 block: outputs 2 V q + V h .. of a lane's row.  A lane holds four outputs of a row and its partner
@@ -521,10 +539,9 @@ __device__ __forceinline__ void finish(const f32x16 (&acc)[NI][MI], const LowRan
     if (lr.t != nullptr && mb < m1) {
       const Owner o = own.whole ? own : owner_of(sg, InMemory{sg}, mb, mb + 32 < m1 ? mb + 32 : m1);
       if (!DROP) {
-        low_rank<T, NI>(sum, lr, sg, o, Nn, m1, mb, nw, lane);
+        low_rank<T, NI>(sum, lr, sg, InMemory{sg}, o, Nn, m1, mb, nw, lane, []() {});
       } else {
-#pragma unroll
-        for (int n = 0; n < NI; ++n) sum[n] += masked_low_rank<T>(lr, sg, ka, key, o, Nn, m1, mb, nw + n * 32, lane);
+        masked_low_rank<T, NI>(sum, lr, sg, InMemory{sg}, ka, key, o, Nn, m1, mb, nw, lane);
       }
     }
     const int row = mb + (lane & 31);
@@ -540,7 +557,7 @@ __device__ __forceinline__ void finish(const f32x16 (&acc)[NI][MI], const LowRan
 }
 
 template <typename T, int BM, int BN, int WGM, int WGN, bool DROP>
-__global__ __launch_bounds__(64 * WGM * WGN) void k_project(const T* __restrict__ X, long long ldx, int Kk, const T* __restrict__ W,
+__global__ __launch_bounds__(64 * WGM * WGN, 2) void k_project(const T* __restrict__ X, long long ldx, int Kk, const T* __restrict__ W,
                                                             long long ldw, int Nn, const T* __restrict__ bias, LowRank lr, Segs sg,
                                                             KeepArgs ka, T* __restrict__ out, long long ldo, int tiles_n) {
   constexpr int NT = 64 * WGM * WGN, MI = BM / WGM / 32, NI = BN / WGN / 32, V = Lines<T>::V, KB = Lines<T>::KB;
@@ -720,6 +737,14 @@ __device__ __forceinline__ void mma_sums(int n, int m, float a, float b) {
   asm volatile("v_mfma_f32_32x32x2_f32 a[%2:%3], %0, %1, a[%2:%3]" ::"v"(a), "v"(b), "i"(16 * (4 * n + m)), "i"(16 * (4 * n + m) + 15));
 }
 
+// the same of fragments that vector instructions have just written: those must lie two wait states back
+__device__ __forceinline__ void mma_sums_late(int n, int m, bf16x8 a, bf16x8 b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 a[%2:%3], %0, %1, a[%2:%3]" ::"v"(a), "v"(b), "i"(16 * (4 * n + m)), "i"(16 * (4 * n + m) + 15));
+}
+__device__ __forceinline__ void mma_sums_late(int n, int m, float a, float b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 a[%2:%3], %0, %1, a[%2:%3]" ::"v"(a), "v"(b), "i"(16 * (4 * n + m)), "i"(16 * (4 * n + m) + 15));
+}
+
 // the low-rank term of row blocks FIRST .. LAST - 1 of a wave's 128 x 128 outputs, which belong to adapter a, added where the sums are
 template <typename T, int FIRST, int LAST>
 __device__ __forceinline__ void low_rank_here(const LowRank& lr, int a, int Nn, int m1, int mw, int nw, int lane) {
@@ -778,7 +803,7 @@ __device__ __forceinline__ void low_rank_here(const LowRank& lr, int a, int Nn, 
           for (int m = 0; m < MB; ++m)
 #pragma unroll
             for (int n = 0; n < 2; ++n)
-              mma_sums(n2 + n, FIRST + m, __builtin_bit_cast(uint4, part == 2 ? bl[n] : bh[n]), __builtin_bit_cast(uint4, part == 0 ? lo[m] : hi[m]), bf16());
+              mma_sums_late(n2 + n, FIRST + m, __is_same(T, f16) && part == 1 ? bl[n] : bh[n], part == 0 ? lo[m] : hi[m]);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
@@ -787,7 +812,7 @@ __device__ __forceinline__ void low_rank_here(const LowRank& lr, int a, int Nn, 
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
-          for (int n = 0; n < 4; ++n) mma_sums(n, FIRST + m, __builtin_bit_cast(f32x4, b[n])[j], in ? t4[m][0][j] : 0.f);
+          for (int n = 0; n < 4; ++n) mma_sums_late(n, FIRST + m, __builtin_bit_cast(f32x4, b[n])[j], in ? t4[m][0][j] : 0.f);
     }
   }
 }
@@ -1028,26 +1053,21 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
         }
       }
 #undef HM_BLOCK
+      if (DROP ? lr.t != nullptr : open >> (k >> 2) & 1) {       // a mask, or several requests' rows
+        const Owner o = own.whole ? own : owner(mb, mb + 32 < m1 ? mb + 32 : m1, ln);
+        auto add = [&](const auto& of) {
+          if constexpr (DROP) masked_low_rank<T, PAIR>(sum, lr, sg, of, ka, key, o, Nn, m1, mb, nb, ln);
+          else low_rank<T, PAIR>(sum, lr, sg, of, o, Nn, m1, mb, nb, ln, []() {});
+        };
+        if (cached) add(InLds{sg, starts, ln});
+        else add(InMemory{sg});
+      }
       if (bias != nullptr) {                          // a lane's outputs are nb + 32 e + 8 (j / 4) + 4 h + j % 4
         const float* b = sb[turn] + nb - n0 + 4 * h;
 #pragma unroll
         for (int e = 0; e < PAIR; ++e)
 #pragma unroll
           for (int j = 0; j < 16; ++j) sum[e][j] += b[e * 32 + 8 * (j >> 2) + (j & 3)];
-      }
-      if (DROP ? lr.t != nullptr : open >> (k >> 2) & 1) {       // a mask, or several requests' rows
-        const Owner o = own.whole ? own : owner(mb, mb + 32 < m1 ? mb + 32 : m1, ln);
-#pragma unroll
-        for (int e = 0; e < PAIR; ++e) {
-          if (nb + e * 32 >= Nn) break;
-          if (DROP) {
-            sum[e] += masked_low_rank<T>(lr, sg, ka, key, o, Nn, m1, mb, nb + e * 32, ln);
-          } else {
-            f32x16 one[1] = {sum[e]};
-            low_rank<T, 1>(one, lr, sg, o, Nn, m1, mb, nb + e * 32, ln);
-            sum[e] = one[0];
-          }
-        }
       }
 #pragma unroll
       for (int e = 0; e < PAIR; ++e)
@@ -1335,27 +1355,53 @@ __device__ __forceinline__ void list_requests(const Segs& sg, int a, int base, R
   __syncthreads();
 }
 
-// sums the slots of an adapter, in order of requests and runs
+// sums the slots of an adapter, in order of requests and runs: their numbers are listed first, so that many loads are under way
+constexpr int SLOTS = 2048;
 template <typename T, int RT>
 __global__ __launch_bounds__(256) void k_outer_sum(Outer oa, Outer ob, Segs sg, int rank, int rows_per_run) {
   __shared__ ReqList list;
+  __shared__ int slot[SLOTS], total[2][256];
   const Outer& o = blockIdx.z == 0 ? oa : ob;
   const int chunks = (rank + 63) / 64, parts = 8 * RT / 4;      // four tiles a workgroup
   const int a = blockIdx.y, per = o.blocks * chunks * parts;
   if ((int)blockIdx.x >= per) return;
   const int pb = blockIdx.x / (chunks * parts), rc = blockIdx.x / parts % chunks, tile = blockIdx.x % parts * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, tid = threadIdx.x;
+  const f32x4* at = reinterpret_cast<const f32x4*>(o.part) + part_at<RT>(o, 0, pb, rc, chunks) + tile * 64 + lane;
+  const size_t step = part_at<RT>(o, 1, 0, 0, chunks);
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   for (int base = 0; base < sg.S; base += 256) {
     list_requests(sg, a, base, &list);
-    for (int e = 0; e < list.n; ++e) {
-      const int q = list.q[e];
-      const int lo = sg.row_start[q] > 0 ? sg.row_start[q] : 0, hi = sg.row_start[q + 1] < sg.M ? sg.row_start[q + 1] : sg.M;
-      if (lo >= hi) continue;
-      const int last = (hi - 1) / rows_per_run;
-#pragma unroll 4
-      for (int run = lo / rows_per_run; run <= last; ++run)
-        v += reinterpret_cast<const f32x4*>(o.part)[part_at<RT>(o, run + q, pb, rc, chunks) + tile * 64 + lane];
+    // runs of request `tid` of the list, and how many come before
+    int first = 0, count = 0;
+    if (tid < list.n) {
+      const int q = list.q[tid], lo = sg.row_start[q] > 0 ? sg.row_start[q] : 0, hi = sg.row_start[q + 1] < sg.M ? sg.row_start[q + 1] : sg.M;
+      if (lo < hi) { first = lo / rows_per_run; count = (hi - 1) / rows_per_run - first + 1; }
+    }
+    total[0][tid] = count;
+    __syncthreads();
+    int now = 0;
+    for (int d = 1; d < 256; d <<= 1) {
+      total[now ^ 1][tid] = total[now][tid] + (tid >= d ? total[now][tid - d] : 0);
+      now ^= 1;
+      __syncthreads();
+    }
+    const int all = total[now][255], before = total[now][tid] - count;
+    for (int b0 = 0; b0 < all; b0 += SLOTS) {
+      for (int i = 0; i < count; ++i)
+        if (before + i >= b0 && before + i < b0 + SLOTS) slot[before + i - b0] = first + i + list.q[tid];
+      __syncthreads();
+      const int n = all - b0 < SLOTS ? all - b0 : SLOTS;
+      int i = 0;
+      for (; i + 8 <= n; i += 8) {
+        f32x4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = at[step * slot[i + u]];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v += x[u];
+      }
+      for (; i < n; ++i) v += at[step * slot[i]];
+      __syncthreads();
     }
   }
   outer_store<T, RT>(o, v, tile, lane, a, pb, 64 * rc, rank);
@@ -1415,14 +1461,27 @@ template <typename T> __global__ __launch_bounds__(256) void k_turn(Turns all) {
   const int id = blockIdx.x - jb.first, bx = id % jb.across, by = id / jb.across % jb.down, z = id / (jb.across * jb.down);
   const T* i = static_cast<const T*>(jb.in) + z * jb.si;
   T* o = static_cast<T*>(jb.out) + z * jb.so;
-  const int c0 = bx * 64, r0 = by * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-#pragma unroll 4
-  for (int j = ty; j < 64; j += 4)
-    tile[j][tx] = r0 + j < jb.rows && c0 + tx < jb.cols ? i[(r0 + j) * jb.ldi + c0 + tx] : (T)0.f;
+  const int c0 = bx * 64, r0 = by * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;    // eight values a thread
+#pragma unroll
+  for (int j = y; j < 64; j += 32) {
+    const int n = r0 + j < jb.rows ? jb.cols - c0 - x : 0;
+    const T* p = i + (r0 + j) * jb.ldi + c0 + x;
+    Frag8<T> f;
+    if (n >= 8) f = frag_load(p);
+    else f = frag_load(p, n);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tile[j][x + e] = f.v[e];
+  }
   __syncthreads();
-#pragma unroll 4
-  for (int j = ty; j < 64; j += 4)
-    if (c0 + j < jb.cols && r0 + tx < jb.ldo) o[(c0 + j) * jb.ldo + r0 + tx] = tile[tx][j];
+#pragma unroll
+  for (int j = y; j < 64; j += 32) {
+    if (c0 + j < jb.cols && r0 + x < jb.ldo) {         // ldo is a multiple of eight
+      Pack8<T> u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u.v[e] = tile[x + e][j];
+      *reinterpret_cast<Pack8<T>*>(o + (c0 + j) * jb.ldo + r0 + x) = u;
+    }
+  }
 }
 
 // ---- host side

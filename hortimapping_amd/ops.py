@@ -118,6 +118,18 @@ def _on(device):
     return _HERE if here else torch.cuda.device(device), torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _of_one_stream(y, stream):
+    """y, a result whose backward pass hands gradients to leaves.  A leaf's node belongs to the stream on which the oldest
+    living graph of that leaf was made, and the backward pass waits across streams: within a capture that pulls the older stream
+    into it, and the process ends when the capture does.  So a node keeps its stream, and a capture on another is refused."""
+    for node, _ in y.grad_fn.next_functions:
+        if hasattr(node, "variable") and node.metadata.setdefault("hortimapping_stream", stream) != stream \
+                and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a graph of the same leaves made on another stream is alive: its backward pass cannot be captured beside "
+                               "it (drop or detach the results of the earlier calls first)")
+    return y
+
+
 def _dropout_forward(x, relu, draws):
     p, seed, word, tag, row0 = draws
     rows, cols, ld = _rows("x", x)
@@ -166,7 +178,7 @@ def dropout(x: torch.Tensor, p: float, seed, *, tag: int = 0, row0: int = 0, rel
     _check_float("x", x)
     draws = _check_draws(p, seed, tag, row0, x.device)
     if torch.is_grad_enabled() and x.requires_grad:
-        return _Dropout.apply(x, bool(relu), draws)
+        return _of_one_stream(_Dropout.apply(x, bool(relu), draws), torch._C._cuda_getCurrentRawStream(x.device.index))
     return _dropout_forward(x, bool(relu), draws)
 
 
@@ -230,7 +242,8 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, A: torch.Tensor, B: to
     all of one type (float32 / float16 / bfloat16) on one GPU.  scale (adapters,) float32, default 1.  Request q holds the
     rows row_start[q] .. row_start[q + 1] - 1 (int32, ascending, S + 1 of them) and uses adapter[q] (int32, S); a value
     outside 0 .. adapters - 1, and rows of no request, get the bare projection.  Both are read on the GPU, when the kernels
-    run: a captured graph may be replayed with others.  p, seed, tag, row0: dropout on the adapters' input, the mask of
+    run: a captured graph may be replayed with others.  (Before a capture with a backward pass, drop the results of eager
+    calls with the same leaves: beside a living one the call is refused.)  p, seed, tag, row0: dropout on the adapters' input, the mask of
     `dropout(x, p, seed, tag=tag, row0=row0)`.  Ranks up to 256, K and N up to 65536."""
     _check_float("x", x)
     for name, t in (("weight", weight), ("A", A), ("B", B)) + ((("bias", bias),) if bias is not None else ()):
@@ -261,5 +274,6 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, A: torch.Tensor, B: to
                 raise ValueError(f"{name} requires a gradient, but the shared projection is frozen: adapter_linear gives "
                                  "gradients of x, A and B (detach it)")
         if x.requires_grad or A.requires_grad or B.requires_grad:
-            return _AdapterLinear.apply(x, A, B, weight, bias, scale, row_start, adapter, draws)
+            return _of_one_stream(_AdapterLinear.apply(x, A, B, weight, bias, scale, row_start, adapter, draws),
+                                  torch._C._cuda_getCurrentRawStream(x.device.index))
     return _adapter_forward(x, weight, bias, A, B, scale, row_start, adapter, draws)[0]

@@ -321,3 +321,107 @@ def test_refusals():
     from hortimapping_amd._lib import HortiHipError
     with pytest.raises(HortiHipError, match="rank 300"):
         ops.adapter_linear(**{**base, "A": r[0], "B": r[1]})
+
+
+# enough tiles for the kernel that goes from tile to tile (256 x 256 outputs): rows, K, N, rank, requests, adapters
+WIDE = {
+    "whole tiles": (16384, 512, 512, 8, [2048] * 8, [0, 1, 2, 0, 1, 2, -1, 0], 3),
+    "ragged": (20001, 512, 515, 16, [1, 4999, 0, 37, 5000, 963, 6000, 2501], [0, 1, 2, 3, -1, 2, 1, 0], 4),
+    "odd reduction": (30000, 259, 512, 5, [10000, 7, 9000, 10900], [2, 0, 1, 2], 3),
+    "short tail": (20000, 66, 512, 12, [9999, 9999], [1, 0], 2),
+    "odd outputs": (70000, 130, 253, 16, [30000, 20000, 20000], [0, 1, 0], 2),
+    "big rank": (16500, 256, 512, 70, [8000, 8500], [1, 0], 2),
+    "rank 64": (16640, 192, 640, 64, [130] * 128, [i % 5 for i in range(128)], 5),
+    "many requests": (20480, 128, 512, 4, [40] * 512, [i % 7 - 1 for i in range(512)], 6),
+}
+
+
+def test_these_sizes_take_the_wide_tiles():
+    """What the cases below are for; the sizes are those of include's rule, restated."""
+    for rows, k, n, r, lengths, which, na in WIDE.values():
+        assert -(-rows // 256) * -(-n // 256) >= 128 and sum(lengths) <= rows and len(lengths) == len(which)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", sorted(WIDE))
+def test_wide_tiles(name, dtype):
+    Case(*WIDE[name], dtype, seed=5).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["whole tiles", "ragged", "odd outputs", "rank 64", "many requests"])
+def test_wide_tiles_with_dropout(name, dtype):
+    Case(*WIDE[name], dtype, seed=6).check(p=0.3, seed=(1 << 40) + 3, tag=1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_wide_tiles_keep_an_infinity_in_its_request(dtype):
+    lengths = [4000, 2, 6000, 6382]
+    c = Case(16384, 128, 512, 8, lengths, [0, 1, 2, 0], 3, dtype)
+    clean = [v.detach().clone() for v in c.check()]
+    ra = torch.from_numpy(AO.segment_of_rows(c.start, c.which, c.rows, 3)).cuda()
+    with torch.no_grad():
+        c.A[1].fill_(float("nan"))
+        c.B[1].fill_(float("inf"))
+        c.x[5000, 7] = float("nan")
+    y = c.call()
+    dx, dA, dB = torch.autograd.grad(y, (c.x, c.A, c.B), c.dy)
+    fine = ra != 1
+    assert torch.equal(dx[fine], clean[1][fine])
+    fine[5000] = False
+    assert torch.equal(y[fine], clean[0][fine]) and bool((~torch.isfinite(y[ra == 1])).all())
+    assert torch.equal(dA[0], clean[2][0]) and torch.equal(dB[0], clean[3][0])
+
+
+def test_wide_tiles_in_a_graph_and_on_two_streams():
+    cs = [Case(*WIDE["ragged"], torch.bfloat16, seed=i) for i in range(2)]
+
+    def step(c):
+        y = c.call(p=0.1, seed=4)
+        return [y] + list(torch.autograd.grad(y, (c.x, c.A, c.B), c.dy))
+    want = [[v.detach() for v in step(c)] for c in cs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cs], []
+    for _ in range(2):
+        for c, s in zip(cs, streams):
+            with torch.cuda.stream(s):
+                got.append(step(c))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+    del got
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(cs[0])
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step(cs[0])))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [64, 65, 129, 256, 257])
+def test_few_rows_and_one_more(rows, dtype):
+    Case(rows, 384, 272, 16, [1] * (rows - 3), [i % 9 - 1 for i in range(rows - 3)], 8, dtype).check(backward=False)
+    Case(rows, 131, 77, 3, [rows // 2, rows - rows // 2], [1, 0], 2, dtype).check(backward=False)
+
+
+def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
+    c = Case(300, 64, 48, 4, [100, 150], [0, 1], 2, torch.float32)
+    y = c.call()
+    z = ops.dropout(c.x, 0.2, 3)
+    want = [v.detach() for v in torch.autograd.grad(y, (c.x, c.A, c.B), c.dy, retain_graph=True)]
+    torch.cuda.synchronize()
+    for call in (c.call, lambda: ops.dropout(c.x, 0.2, 3)):
+        g = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="another stream"):
+            with torch.cuda.graph(g):
+                call()
+    del y, z
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = torch.autograd.grad(c.call(), (c.x, c.A, c.B), c.dy)
+    for _ in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))

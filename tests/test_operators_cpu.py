@@ -1,6 +1,7 @@
 """CPU tests of dropout and the adapters beside a projection: the oracle's generator against the published vectors, the
 struct's layout, and what the entry points refuse (no GPU needed: nothing is launched)."""
 import ctypes
+import gc
 import os
 import subprocess
 import tempfile
@@ -140,3 +141,20 @@ def test_rows_that_are_refused(shape, strides):
     with pytest.raises(ValueError):
         ops._rows("x", t)
     assert ops._rows_of_grad(t)[1:] == (int(np.prod(shape[:-1])), shape[-1], shape[-1])
+
+
+def test_a_leaf_of_another_stream_is_refused_within_a_capture(monkeypatch):
+    x = torch.zeros(3, requires_grad=True)
+    y = ops._of_one_stream(x * 2, 7)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert ops._of_one_stream(x * 3, 8).shape == (3,)                         # no capture: nothing to refuse
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    assert ops._of_one_stream(x * 3, 7).shape == (3,)
+    with pytest.raises(RuntimeError, match="another stream"):
+        ops._of_one_stream(x * 3, 8)
+    del y
+    gc.collect()                                                              # (the refusal's traceback held its argument)
+    assert ops._of_one_stream(x * 3, 8).shape == (3,)                         # the older graph is gone
+    h = torch.zeros(3, requires_grad=True) * 1
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    ops._of_one_stream(h * 2, 1), ops._of_one_stream(h * 2, 2)                # no leaf: its nodes are not looked at
