@@ -8,6 +8,18 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 namespace hm {
 
+// a * b, rounded, also where it is added to something: which products of a sum of three join a fused multiply-add is otherwise
+// the compiler's choice and moves with its options, and with it the last bit of a transformed point or a Jacobian
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+// a0 * b0 + a1 * b1 + a2 * b2 with the third product rounded
+__device__ __forceinline__ float dot3_third_rounded(float a0, float b0, float a1, float b1, float a2, float b2) {
+  return fmaf(a0, b0, a1 * b1) + rounded_product(a2, b2);
+}
+
+
 constexpr int HID = 512;        // hidden width of the DeepSDF decoder (specs.json:8)
 constexpr int TQ = 64;          // decoder queries per workgroup tile (2 MFMA N-blocks of 32)
 constexpr int NWAVE = 8;        // waves per decoder workgroup

@@ -542,7 +542,7 @@ __global__ __launch_bounds__(512, 2) void k_decoder_h(const DecodeArgsH a) {
       row[3] = g2 * p[1] - g1 * p[2];
       row[4] = g0 * p[2] - g2 * p[0];
       row[5] = g1 * p[0] - g0 * p[1];
-      if (sg.pose_dim == 7) row[6] = g0 * p[0] + g1 * p[1] + g2 * p[2];
+      if (sg.pose_dim == 7) row[6] = hm::dot3_third_rounded(g0, p[0], g1, p[1], g2, p[2]);
     }
   }
 }

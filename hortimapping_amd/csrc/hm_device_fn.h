@@ -30,7 +30,12 @@ __device__ inline void exp_pose(const float* x, bool sim3, float* T) {
   const float W[9] = {0.f, -w[2], w[1], w[2], 0.f, -w[0], -w[1], w[0], 0.f};
   float W2[9];
   mat3_mul(W, W, W2);
-  const float theta = sqrtf(w[0] * w[0] + w[1] * w[1] + w[2] * w[2]);
+  // the squares are rounded before they are added (one of them is not): what the compiler would fuse here moves with its options
+  const float w00 = rounded_product(w[0], w[0]), w11 = rounded_product(w[1], w[1]), w22 = rounded_product(w[2], w[2]);
+  W2[0] = -w11 - w22;
+  W2[4] = fmaf(-w[0], w[0], -w22);
+  W2[8] = -w00 - w11;
+  const float theta = sqrtf(w00 + w11 + w22);
   const float th2 = theta * theta;
   const float st = sinf(theta), ct = cosf(theta);
   const float es = sim3 ? expf(s) : 1.f;
@@ -57,7 +62,7 @@ __device__ inline void exp_pose(const float* x, bool sim3, float* T) {
   }
   for (int i = 0; i < 3; ++i) {
     for (int j = 0; j < 3; ++j) T[i * 4 + j] = es * R[i * 3 + j];
-    T[i * 4 + 3] = Jm[i * 3 + 0] * v[0] + Jm[i * 3 + 1] * v[1] + Jm[i * 3 + 2] * v[2];
+    T[i * 4 + 3] = dot3_third_rounded(Jm[i * 3 + 0], v[0], Jm[i * 3 + 1], v[1], Jm[i * 3 + 2], v[2]);
   }
   T[12] = 0.f; T[13] = 0.f; T[14] = 0.f; T[15] = 1.f;
 }
@@ -70,7 +75,7 @@ __device__ __forceinline__ float huber_rho(float r, float th) {
   if (th <= 0.f) return 1.f;          // robust kernel off (before robust_iter, mask term)
   if (a == 0.f) return 0.f;
   if (a <= th) return 1.f;
-  return (2.f * th * a - th * th) / (a * a);
+  return fmaf(-th, th, 2.f * th * a) / (a * a);       // (which of the two products is rounded is not left to the compiler)
 }
 
 }  // namespace hm
