@@ -19,6 +19,7 @@
 #include "hm_internal.h"
 #include "hm_keep.h"
 #include "../../include/hortimapping_amd.h"
+#include "../../include/hortimapping_amd_debug.h"
 
 using namespace hm;
 
@@ -1612,6 +1613,8 @@ int pick_tile(long long rows, int n, int k, int size) {
   return k >= line && tiles(256) >= 64 && wide < other ? 256 : small;
 }
 
+int g_tile = 0;            // hm_debug_set_adapter_tile
+
 template <typename T>
 int project(const hm_adapter_args& g, const T* X, long long ldx, int Kk, const T* W, long long ldw, int Nn, const T* bias,
             const LowRank& lr, bool drop, const KeepArgs& ka, T* out, long long ldo, hipStream_t st) {
@@ -1619,13 +1622,14 @@ int project(const hm_adapter_args& g, const T* X, long long ldx, int Kk, const T
 #define HM_GO(BM, BN, WGM, WGN, D)                                                                                                   \
   hipLaunchKernelGGL((k_project<T, BM, BN, WGM, WGN, D>), dim3((unsigned)(((g.rows + BM - 1) / BM) * ((Nn + BN - 1) / BN))),         \
                      dim3(64 * WGM * WGN), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, (Nn + BN - 1) / BN)
-  const int tile = pick_tile(g.rows, Nn, Kk, sizeof(T));
+  int tile = pick_tile(g.rows, Nn, Kk, sizeof(T));
+  if (g_tile != 0 && (g_tile != WIDE || Kk >= Lines<T>::KB)) tile = g_tile;
   if (tile == 256) {
     const int tm = (int)((g.rows + WIDE - 1) / WIDE), tn = (Nn + WIDE - 1) / WIDE;
     const dim3 grid((long long)tm * tn < 256 ? tm * tn : 256);
     if (drop) hipLaunchKernelGGL((k_project_wide<T, true>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, tm, tn);
     else hipLaunchKernelGGL((k_project_wide<T, false>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, tm, tn);
-  } else if (tile == 128) {
+  } else if (tile == 128 && sizeof(T) == 2) {
     if constexpr (sizeof(T) == 2) { if (drop) HM_GO(128, 128, 2, 2, true); else HM_GO(128, 128, 2, 2, false); }
   } else {
     if (drop) HM_GO(64, 64, 2, 2, true); else HM_GO(64, 64, 2, 2, false);
@@ -1645,7 +1649,7 @@ template <typename T> int forward(const hm_adapter_args& g, const KeepArgs& ka, 
     if (rc) return rc;
   }
   const LowRank lr = {any ? d_t : nullptr, g.d_b, (long long)g.n * g.rank, g.rank, g.rank, pad8(g.rank)};
-  if (g.rows <= FEW_ROWS) {
+  if (g.rows <= FEW_ROWS && g_tile == 0) {
     const dim3 grid((g.n + 15) / 16, (unsigned)((g.rows + 63) / 64));
     const Segs sg = segs_of(g);
 #define HM_GO(MT) hipLaunchKernelGGL((k_project_few<T, MT>), grid, dim3(64 * FEW_WAVES), 0, st, X, g.ld_x, g.k, W, g.ld_w, g.n, bias, lr, sg, y, ld_y)
@@ -1712,6 +1716,8 @@ int backward(const hm_adapter_args& g, const KeepArgs& ka, const void* d_dy, lon
 }
 
 }  // namespace
+
+extern "C" void hm_debug_set_adapter_tile(int tile) { g_tile = tile == 64 || tile == 128 || tile == WIDE ? tile : 0; }
 
 extern "C" int hm_adapter_linear(const hm_adapter_args* g, void* d_y, long long ld_y, float* d_t, void* stream) {
   KeepArgs ka;

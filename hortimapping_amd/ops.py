@@ -199,21 +199,24 @@ def _adapter_forward(x, weight, bias, A, B, scale, row_start, adapter, draws):
     guard, stream = _on(x.device)
     with guard:
         _lib.check(_lib.lib().hm_adapter_linear(ctypes.byref(args), y.data_ptr(), n, t.data_ptr(), stream), "hm_adapter_linear")
-    return y, t, args
+    return y, t
 
 
 class _AdapterLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, A, B, weight, bias, scale, row_start, adapter, draws):
-        y, t, ctx.args = _adapter_forward(x, weight, bias, A, B, scale, row_start, adapter, draws)
-        ctx.save_for_backward(x, A, B, weight, scale, row_start, adapter, t, draws[2])
+        y, t = _adapter_forward(x, weight, bias, A, B, scale, row_start, adapter, draws)
+        p, seed, word, tag, row0 = draws
+        ctx.draws = p, seed, tag, row0
+        ctx.save_for_backward(x, A, B, weight, scale, row_start, adapter, t, word)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, A, B, _, _, _, _, t, _ = ctx.saved_tensors        # ctx.args points into these: unchanged, or this line raises
-        args = ctx.args
+        x, A, B, weight, scale, row_start, adapter, t, word = ctx.saved_tensors      # (hooks may have moved them meanwhile)
+        p, seed, tag, row0 = ctx.draws
+        args = _adapter_args(x, weight, None, A, B, scale, row_start, adapter, (p, seed, word, tag, row0))
         dy, _, _, ld = _rows_of_grad(dy)
         want_x, want_a, want_b = ctx.needs_input_grad[:3]
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None

@@ -33,6 +33,8 @@ int hm_workspace_set_k4_split(hm_workspace_t ws, int on);
 void hm_debug_set_trace(long long* d_buf);      /* [NSTAGE * 8 + 1] or NULL (the product kernel writes [NSTAGE * 4 + 1] of it) */
 void hm_debug_set_k5_trace(long long* d_buf);   /* [32] or NULL */
 void hm_debug_force_direct_solve(int on);        /* tests: 1 = every solve takes the blocked-Cholesky fallback of K5 */
+void hm_debug_set_adapter_tile(int tile);       /* 64, 128 (16-bit types) or 256: outputs a side of a tile of hm_adapter_linear and its
+                                                   backward pass, whatever the sizes (256: reductions of 128 bytes on); else: the rule */
 void hm_debug_set_trace_thread(int tid);         /* which thread of workgroup 0 writes the hm_debug_set_trace stamps */
 void hm_debug_split_render(int on);              /* A/B + tests: 1 = the f16x3 render chain as separate launches with a
                                                   * forward+backward Jacobian pass (round 2) instead of the fused grid +

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import adapter_oracle as AO
-from hortimapping_amd import ops
+from hortimapping_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -323,7 +323,44 @@ def test_refusals():
         ops.adapter_linear(**{**base, "A": r[0], "B": r[1]})
 
 
-# enough tiles for the kernel that goes from tile to tile (256 x 256 outputs): rows, K, N, rank, requests, adapters
+@pytest.fixture
+def tile():
+    yield _lib.lib().hm_debug_set_adapter_tile
+    _lib.lib().hm_debug_set_adapter_tile(0)
+
+
+@pytest.mark.parametrize("side", [64, 128, 256])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", sorted(LAYOUTS))
+def test_every_tile_on_every_layout(tile, name, dtype, side):
+    tile(side)
+    Case(*LAYOUTS[name], dtype, seed=9).check()
+
+
+@pytest.mark.parametrize("side", [64, 128, 256])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["ragged", "short", "tile crossing", "big rank", "wide"])
+def test_every_tile_with_dropout(tile, name, dtype, side):
+    tile(side)
+    Case(*LAYOUTS[name], dtype, seed=10).check(p=0.3, seed=77, tag=2)
+
+
+@pytest.mark.parametrize("side", [64, 128, 256])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_tile_with_hundreds_of_requests(tile, dtype, side):
+    tile(side)
+    for n in (255, 256, 700):                             # around what the wide tiles keep at hand
+        Case(3 * n + 5, 130, 72, 6, [i % 7 for i in range(n)], [i % 6 - 1 for i in range(n)], 5, dtype, seed=n).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_reduction_at_the_wide_tile(tile, dtype):
+    tile(256)
+    for k in list(range(64, 75)) + [127, 128, 129, 191, 255]:
+        Case(70, k, 40, 9, [33, 30], [0, 1], 2, dtype, seed=k).check()
+
+
+# many tiles a workgroup, at whatever tile: rows, K, N, rank, lengths, adapters used, adapters
 WIDE = {
     "whole tiles": (16384, 512, 512, 8, [2048] * 8, [0, 1, 2, 0, 1, 2, -1, 0], 3),
     "ragged": (20001, 512, 515, 16, [1, 4999, 0, 37, 5000, 963, 6000, 2501], [0, 1, 2, 3, -1, 2, 1, 0], 4),
@@ -336,26 +373,23 @@ WIDE = {
 }
 
 
-def test_these_sizes_take_the_wide_tiles():
-    """What the cases below are for; the sizes are those of include's rule, restated."""
-    for rows, k, n, r, lengths, which, na in WIDE.values():
-        assert -(-rows // 256) * -(-n // 256) >= 128 and sum(lengths) <= rows and len(lengths) == len(which)
-
-
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("name", sorted(WIDE))
-def test_wide_tiles(name, dtype):
+def test_wide_tiles(tile, name, dtype):
+    tile(256)
     Case(*WIDE[name], dtype, seed=5).check()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("name", ["whole tiles", "ragged", "odd outputs", "rank 64", "many requests"])
-def test_wide_tiles_with_dropout(name, dtype):
+def test_wide_tiles_with_dropout(tile, name, dtype):
+    tile(256)
     Case(*WIDE[name], dtype, seed=6).check(p=0.3, seed=(1 << 40) + 3, tag=1)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_wide_tiles_keep_an_infinity_in_its_request(dtype):
+def test_wide_tiles_keep_an_infinity_in_its_request(tile, dtype):
+    tile(256)
     lengths = [4000, 2, 6000, 6382]
     c = Case(16384, 128, 512, 8, lengths, [0, 1, 2, 0], 3, dtype)
     clean = [v.detach().clone() for v in c.check()]
@@ -373,7 +407,8 @@ def test_wide_tiles_keep_an_infinity_in_its_request(dtype):
     assert torch.equal(dA[0], clean[2][0]) and torch.equal(dB[0], clean[3][0])
 
 
-def test_wide_tiles_in_a_graph_and_on_two_streams():
+def test_wide_tiles_in_a_graph_and_on_two_streams(tile):
+    tile(256)
     cs = [Case(*WIDE["ragged"], torch.bfloat16, seed=i) for i in range(2)]
 
     def step(c):
@@ -425,3 +460,22 @@ def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_saved_tensors_that_were_moved_away(dtype):
+    c = Case(300, 72, 48, 5, [100, 150], [0, 1], 2, dtype)
+
+    def run(hooks):
+        with hooks:
+            h = c.x * 1
+            y = ops.dropout(ops.adapter_linear(h, c.W * 1, c.A, c.B, c.row_start + 0, c.adapter + 0, bias=c.b, scale=c.scale * 1, p=0.2, seed=3),
+                            0.3, 5, relu=True)
+            del h
+        junk = [torch.full_like(c.x, float("nan")) for _ in range(4)]
+        out = torch.autograd.grad(y, (c.x, c.A, c.B), c.dy)
+        del junk
+        return out
+    import contextlib
+    for a, b in zip(run(torch.autograd.graph.save_on_cpu()), run(contextlib.nullcontext())):
+        assert torch.equal(a, b)
