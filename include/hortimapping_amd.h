@@ -365,7 +365,8 @@ int hm_dropout_backward(const void* d_dy, long long ld_dy, const void* d_y, long
  * seed / d_seed / tag / row0.  row_start and adapter are device arrays that the host never reads: a row_start that does not
  * ascend gives unspecified values for the rows concerned, nothing else.
  * A row's result depends on its own row and adapter alone (not on the batch around it, bit for bit as long as the same kernels
- * run; an infinity or NaN in another request or adapter does not reach it). */
+ * run; an infinity or NaN in another request or adapter does not reach it).  An infinity among a result's own factors may come out
+ * as NaN: 32-bit values are multiplied in two parts. */
 #define HM_ADAPTER_MAX_ROWS 16777216
 #define HM_ADAPTER_MAX_WIDTH 65536
 #define HM_ADAPTER_MAX_RANK 256
