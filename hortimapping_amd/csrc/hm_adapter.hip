@@ -1343,36 +1343,52 @@ __global__ __launch_bounds__(256) void k_outer(Outer oa, Outer ob, Segs sg, Keep
   outer_run<T, RT>(o, sg, ka, rank, rows_per_run, red);
 }
 
-// requests of an adapter in ascending order, 256 looked at a time
+// requests of an adapter in ascending order, 256 looked at a time (by the first 256 threads)
 struct ReqList { int n; int q[256]; };
 __device__ __forceinline__ void list_requests(const Segs& sg, int a, int base, ReqList* l) {
   __shared__ int cnt[4];
   const int q = base + threadIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const bool is = q < sg.S && sg.adapter[q] == a && sg.row_start[q] < sg.row_start[q + 1];
+  const bool is = w < 4 && q < sg.S && sg.adapter[q] == a && sg.row_start[q] < sg.row_start[q + 1];
   const unsigned long long b = __ballot(is);
   __syncthreads();                                     // the list of the last step is read
-  if (lane == 0) cnt[w] = __popcll(b);
+  if (lane == 0 && w < 4) cnt[w] = __popcll(b);
   __syncthreads();
   int at = 0;
-  for (int i = 0; i < w; ++i) at += cnt[i];
+  for (int i = 0; i < 4; ++i) at += i < w ? cnt[i] : 0;
   if (is) l->q[at + __popcll(b & ((1ull << lane) - 1))] = q;
   if (threadIdx.x == 0) l->n = cnt[0] + cnt[1] + cnt[2] + cnt[3];
   __syncthreads();
 }
 
-// sums the slots of an adapter, in order of requests and runs: their numbers are listed first, so that many loads are under way
+// n <= 8 values side by side
+template <typename T> struct alignas(sizeof(T)) Eight { T v[8]; };
+template <typename T> __device__ __forceinline__ void store_eight(T* o, const float (&v)[8], int n) {
+  Eight<T> u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) u.v[j] = (T)v[j];
+  if (n >= 8) {
+    *reinterpret_cast<Eight<T>*>(o) = u;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (j < n) o[j] = u.v[j];
+  }
+}
+
+// sums the slots of an adapter, in order of requests and runs: their numbers are listed first, so that many loads are under way.
+// 128 columns x 16 ranks a workgroup, results out through the LDS: as the products lie, each would be a store of its own
 constexpr int SLOTS = 2048;
 template <typename T, int RT>
-__global__ __launch_bounds__(256) void k_outer_sum(Outer oa, Outer ob, Segs sg, int rank, int rows_per_run) {
+__global__ __launch_bounds__(512) void k_outer_sum(Outer oa, Outer ob, Segs sg, int rank, int rows_per_run) {
   __shared__ ReqList list;
   __shared__ int slot[SLOTS], total[2][256];
+  __shared__ float sums[16][OU_COLS + 1];
   const Outer& o = blockIdx.z == 0 ? oa : ob;
-  const int chunks = (rank + 63) / 64, parts = 8 * RT / 4;      // four tiles a workgroup
+  const int chunks = (rank + 63) / 64, parts = RT;    // eight tiles a workgroup, one a wave
   const int a = blockIdx.y, per = o.blocks * chunks * parts;
   if ((int)blockIdx.x >= per) return;
-  const int pb = blockIdx.x / (chunks * parts), rc = blockIdx.x / parts % chunks, tile = blockIdx.x % parts * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, tid = threadIdx.x;
-  const f32x4* at = reinterpret_cast<const f32x4*>(o.part) + part_at<RT>(o, 0, pb, rc, chunks) + tile * 64 + lane;
+  const int pb = blockIdx.x / (chunks * parts), rc = blockIdx.x / parts % chunks, i16 = blockIdx.x % parts;
+  const int lane = threadIdx.x & 63, tid = threadIdx.x, w = tid >> 6;
+  const f32x4* at = reinterpret_cast<const f32x4*>(o.part) + part_at<RT>(o, 0, pb, rc, chunks) + (w * RT + i16) * 64 + lane;
   const size_t step = part_at<RT>(o, 1, 0, 0, chunks);
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   for (int base = 0; base < sg.S; base += 256) {
@@ -1383,15 +1399,15 @@ __global__ __launch_bounds__(256) void k_outer_sum(Outer oa, Outer ob, Segs sg, 
       const int q = list.q[tid], lo = sg.row_start[q] > 0 ? sg.row_start[q] : 0, hi = sg.row_start[q + 1] < sg.M ? sg.row_start[q + 1] : sg.M;
       if (lo < hi) { first = lo / rows_per_run; count = (hi - 1) / rows_per_run - first + 1; }
     }
-    total[0][tid] = count;
+    if (tid < 256) total[0][tid] = count;
     __syncthreads();
     int now = 0;
     for (int d = 1; d < 256; d <<= 1) {
-      total[now ^ 1][tid] = total[now][tid] + (tid >= d ? total[now][tid - d] : 0);
+      if (tid < 256) total[now ^ 1][tid] = total[now][tid] + (tid >= d ? total[now][tid - d] : 0);
       now ^= 1;
       __syncthreads();
     }
-    const int all = total[now][255], before = total[now][tid] - count;
+    const int all = total[now][255], before = total[now][tid & 255] - count;
     for (int b0 = 0; b0 < all; b0 += SLOTS) {
       for (int i = 0; i < count; ++i)
         if (before + i >= b0 && before + i < b0 + SLOTS) slot[before + i - b0] = first + i + list.q[tid];
@@ -1409,7 +1425,24 @@ __global__ __launch_bounds__(256) void k_outer_sum(Outer oa, Outer ob, Segs sg, 
       __syncthreads();
     }
   }
-  outer_store<T, RT>(o, v, tile, lane, a, pb, 64 * rc, rank);
+  // value q of tile j in a lane: column 8 (4 (lane / 16) + q) + j of the block, rank lane % 16
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sums[lane & 15][8 * (4 * (lane >> 4) + q) + w] = v[q] * o.factor;
+  __syncthreads();
+  if (tid >= 256) return;
+  const int r0 = 64 * rc + 16 * i16;
+  float u[8];
+  if (o.op == 1) {                                    // columns side by side: a thread takes eight of a rank
+    const int r = tid >> 4, c = tid & 15, p = outer_col(o.P, pb, c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = sums[r][8 * c + j];
+    if (r0 + r < rank) store_eight(static_cast<T*>(o.out) + a * o.oa + p + (r0 + r) * o.oi, u, o.P - p);
+  } else {                                            // ranks side by side: eight of a column
+    const int col = tid >> 1, r = 8 * (tid & 1), p = outer_col(o.P, pb, col >> 3) + (col & 7);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = sums[r + j][col];
+    if (p < o.P) store_eight(static_cast<T*>(o.out) + a * o.oa + p * o.op + r0 + r, u, rank - r0 - r);
+  }
 }
 
 // the same without partial sums, for so many requests that their slots would not fit: a workgroup sums all rows of an adapter
@@ -1711,7 +1744,7 @@ int backward(const hm_adapter_args& g, const KeepArgs& ka, const void* d_dy, lon
       hipLaunchKernelGGL((k_outer_direct<T, RT>), dim3(blocks * p.chunks, g.adapters, 2), dim3(256), 0, st, oa, ob, sg, ka, g.rank); \
     } else {                                                                                                                         \
       if (any) hipLaunchKernelGGL((k_outer<T, RT>), dim3(blocks, p.runs, 2), dim3(256), 0, st, oa, ob, sg, ka, g.rank, p.rows_per_run); \
-      hipLaunchKernelGGL((k_outer_sum<T, RT>), dim3(blocks * p.chunks * 2 * RT, g.adapters, 2), dim3(256), 0, st, oa, ob, sg, g.rank, p.rows_per_run); \
+      hipLaunchKernelGGL((k_outer_sum<T, RT>), dim3(blocks * p.chunks * RT, g.adapters, 2), dim3(512), 0, st, oa, ob, sg, g.rank, p.rows_per_run); \
     }
     if (p.rt == 1) { HM_GO(1) } else if (p.rt == 2) { HM_GO(2) } else { HM_GO(4) }
 #undef HM_GO
