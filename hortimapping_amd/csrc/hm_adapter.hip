@@ -864,7 +864,7 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
   constexpr int MI = 4, NI = 4, V = Lines<T>::V, KB = Lines<T>::KB;
   __shared__ uint4 lds[2][2 * WIDE * 8];              // X lines, then W lines
   __shared__ uint4 stage[4][256];                     // 32 lines of results a wave
-  __shared__ float sb[2][WIDE];                       // the bias, of this tile and the next
+  __shared__ float sb[4][WIDE / 2];                   // the bias of each wave's outputs, written and read by that wave alone
   __shared__ int starts[2][LDS_REQUESTS];             // row_start, and the adapter of each request, where they are few
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
   const int lane = tid & 63, l32 = lane & 31, h = lane >> 5;
@@ -927,12 +927,6 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
     if (tid <= sg.S) starts[0][tid] = sg.row_start[tid];
     if (tid < sg.S) starts[1][tid] = sg.adapter[tid];
   }
-  auto bias_of = [&](int of, int half) {
-    int m0, n0;
-    place(of, m0, n0);
-    sb[half][tid] = bias != nullptr && n0 + tid < Nn ? (float)bias[n0 + tid] : 0.f;
-  };
-  bias_of(tile, 0);
   aim();
 #pragma unroll
   for (int j = 0; j < 16; ++j) fetch(j);
@@ -951,7 +945,7 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
     fr[set][i] = lds[buf][(i < 4 ? rw + i * 256 : rx + (i - 4) * 256) + at];
   };
   int buf = 0;
-  for (int turn = 0; tile < end; tile += 32, turn ^= 1) {
+  for (; tile < end; tile += 32) {
     int m0, n0;
     place(tile, m0, n0);
     const int m1 = m0 + WIDE < sg.M ? m0 + WIDE : sg.M;
@@ -961,7 +955,13 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
     Owner own = {0, -1, false};
     if (lr.t != nullptr) own = owner(m0, m1, fresh(tid) & 63);
     sums_clear();
-    if (tile + 32 < end) bias_of(tile + 32, turn ^ 1);
+    // waves finish a tile at different times, with no barrier between that and the next tile: what one of them adds there must not
+    // be written by another
+    if (bias != nullptr) {
+      const int ln = fresh(tid) & 63;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) sb[w][64 * e + ln] = nw + 64 * e + ln < Nn ? (float)bias[nw + 64 * e + ln] : 0.f;
+    }
     // (the last step of the tile before read these too; across its end they would take 32 registers)
 #pragma unroll
     for (int i = 0; i < 8; ++i) read(buf, 0, 0, i);
@@ -1068,7 +1068,7 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
         else add(InMemory{sg});
       }
       if (bias != nullptr) {                          // a lane's outputs are nb + 32 e + 8 (j / 4) + 4 h + j % 4
-        const float* b = sb[turn] + nb - n0 + 4 * h;
+        const float* b = sb[w] + nb - nw + 4 * h;
 #pragma unroll
         for (int e = 0; e < PAIR; ++e)
 #pragma unroll

@@ -360,7 +360,7 @@ def test_every_reduction_at_the_wide_tile(tile, dtype):
         Case(70, k, 40, 9, [33, 30], [0, 1], 2, dtype, seed=k).check()
 
 
-# many tiles a workgroup, at whatever tile: rows, K, N, rank, lengths, adapters used, adapters
+# the wide tile (a tile a workgroup, "odd outputs" two for some): rows, K, N, rank, lengths, adapters used, adapters
 WIDE = {
     "whole tiles": (16384, 512, 512, 8, [2048] * 8, [0, 1, 2, 0, 1, 2, -1, 0], 3),
     "ragged": (20001, 512, 515, 16, [1, 4999, 0, 37, 5000, 963, 6000, 2501], [0, 1, 2, 3, -1, 2, 1, 0], 4),
@@ -479,3 +479,71 @@ def test_saved_tensors_that_were_moved_away(dtype):
     import contextlib
     for a, b in zip(run(torch.autograd.graph.save_on_cpu()), run(contextlib.nullcontext())):
         assert torch.equal(a, b)
+
+
+def tiles_of_workgroups(rows, n):
+    """Columns at which the 256-wide tiles of each workgroup start, in their order (eight runs of tiles, one for each part of the
+    chip; 32 workgroups take turns in a run; bands of eight tiles of rows)."""
+    tm, tn = -(-rows // 256), -(-n // 256)
+    each, extra = divmod(tm * tn, 8)
+    out = []
+    for b in range(min(tm * tn, 256)):
+        part = b % 8
+        first = part * each + min(part, extra)
+        mine = range(first + b // 8, first + each + (part < extra), 32)
+        out.append([t % (8 * tn) // min(8, tm - t // (8 * tn) * 8) * 256 for t in mine])
+    return out
+
+
+# rows, K, N: at least three tiles a workgroup, other columns from one to the next but one
+MANY = {
+    "few rows in the last tile": (16228, 64, 4096),       # 100: two of the four waves have nothing to store there
+    "three tiles of columns": (65536, 64, 768),
+    "six tiles of columns": (24676, 64, 1536),
+    "odd": (20060, 70, 2100),                             # 92 rows and 52 outputs in the last tiles, a tail of the reduction
+    "half a tile of rows": (33000, 96, 1300),             # 232 rows in the last tiles
+}
+
+
+@pytest.mark.parametrize("adapters", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", sorted(MANY))
+def test_many_tiles_a_workgroup(tile, name, dtype, adapters):
+    """Tiles that one workgroup takes one after the other, with a bias that no two blocks of 64 outputs share: in 64 bits on the GPU."""
+    rows, k, n = MANY[name]
+    cols = tiles_of_workgroups(rows, n)
+    assert sum(map(len, cols)) == -(-rows // 256) * -(-n // 256)
+    assert any(len(c) >= 3 and c[i] != c[i + 2] for c in cols for i in range(len(c) - 2))
+    # requests that end in one half of a tile's rows and not in the other, in the last rows too
+    cuts = sorted({0, *range(300, rows, 1111), rows - 40, rows - 3}) if adapters else []
+    lengths = [b - a for a, b in zip(cuts, cuts[1:])]
+    c = Case(rows, k, n, 8, lengths, [i % 4 - 1 for i in range(len(lengths))], 3, dtype, seed=11)
+    c.b = (torch.arange(n, device="cuda") // 64 * 3 - 90).to(dtype)      # whole numbers below 256: exact in every type
+    tile(256)
+    with torch.no_grad():
+        y = c.call()
+        ra = torch.from_numpy(AO.segment_of_rows(c.start, c.which, rows, 3)).cuda()
+        sums = []
+        for f in (lambda v: v.detach().double(), lambda v: v.detach().double().abs()):
+            x, out = f(c.x), f(c.x) @ f(c.W).t() + f(c.b)
+            for i in range(3):
+                m = torch.nonzero(ra == i)[:, 0]
+                out[m] += (x[m] @ f(c.A[i]).t() * f(c.scale[i])) @ f(c.B[i]).t()
+            sums.append(out)
+        want, size = sums
+        f = torch.finfo(dtype)
+        split = 0.0 if dtype == torch.float32 else 2.0 ** -16
+        tol = ((k + 2 * 8 + 8) * 2.0 ** -23 + split) * size + f.eps / 2 * want.abs() + f.smallest_normal * f.eps
+        err = (y.double() - want).abs()
+        assert bool((err <= tol).all()), (float((err / tol).max()), torch.nonzero(err > tol)[:4].tolist())
+        for _ in range(3):
+            assert torch.equal(c.call(), y)
+
+
+@pytest.mark.parametrize("p", [0.0, 0.3])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_of_many_tiles_a_workgroup(tile, dtype, p):
+    """dx has the tiles here: 97 x 6 of them."""
+    assert max(map(len, tiles_of_workgroups(24676, 1536))) == 3
+    tile(256)
+    Case(24676, 1536, 64, 8, [4000, 60, 7000, 1, 9000, 4600], [0, 1, -1, 2, 1, 0], 3, dtype, seed=12).check(p=p, seed=6, tag=3)
