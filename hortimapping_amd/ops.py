@@ -5,6 +5,7 @@ import contextlib
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -109,6 +110,16 @@ def _check_draws(p, seed, tag, row0, device) -> tuple:
     return p, int(seed), word, int(tag), int(row0)
 
 
+def _no_tangents(**tensors) -> None:
+    """Refuses forward-mode derivatives.  A tensor with a tangent does not require a gradient, so a call would compute the value
+    and lose the tangent without a word."""
+    if forward_ad._current_level < 0:                    # outside of every dual_level: no tensor has one
+        return
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} carries a forward-mode tangent, but there are gradients in reverse mode only")
+
+
 _HERE = contextlib.nullcontext()
 
 
@@ -174,8 +185,10 @@ def dropout(x: torch.Tensor, p: float, seed, *, tag: int = 0, row0: int = 0, rel
     column) alone; p is taken to the nearest 2^-16.  `seed`: an int, or an int64 tensor of one element on x's device that is
     read when the kernel runs (change it between replays of a captured graph; not between a forward pass and its backward).
     `tag`: number of the layer, so that one seed a step is enough.  `row0`: number of x's first row, so that a shard or a
-    chunk of a batch draws what the whole batch would.  A NaN that is dropped is dropped: the result there is 0."""
+    chunk of a batch draws what the whole batch would.  A NaN that is dropped is dropped: the result there is 0.
+    Gradients are those of reverse mode, once; an x with a forward-mode tangent is refused."""
     _check_float("x", x)
+    _no_tangents(x=x)
     draws = _check_draws(p, seed, tag, row0, x.device)
     if torch.is_grad_enabled() and x.requires_grad:
         return _of_one_stream(_Dropout.apply(x, bool(relu), draws), torch._C._cuda_getCurrentRawStream(x.device.index))
@@ -247,7 +260,8 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, A: torch.Tensor, B: to
     outside 0 .. adapters - 1, and rows of no request, get the bare projection.  Both are read on the GPU, when the kernels
     run: a captured graph may be replayed with others.  (Before a capture with a backward pass, drop the results of eager
     calls with the same leaves: beside a living one the call is refused.)  p, seed, tag, row0: dropout on the adapters' input, the mask of
-    `dropout(x, p, seed, tag=tag, row0=row0)`.  Ranks up to 256, K and N up to 65536."""
+    `dropout(x, p, seed, tag=tag, row0=row0)`.  Ranks up to 256, K and N up to 65536.
+    Gradients are those of reverse mode, once; tensors with a forward-mode tangent are refused."""
     _check_float("x", x)
     for name, t in (("weight", weight), ("A", A), ("B", B)) + ((("bias", bias),) if bias is not None else ()):
         _check_float(name, t, x)
@@ -270,6 +284,7 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, A: torch.Tensor, B: to
             raise ValueError(f"{name} must be one-dimensional, contiguous int32 on {x.device}")
     if row_start.numel() != adapter.numel() + 1:
         raise ValueError(f"{adapter.numel()} requests need {adapter.numel() + 1} row starts, got {row_start.numel()}")
+    _no_tangents(x=x, weight=weight, A=A, B=B, bias=bias, scale=scale)
     draws = _check_draws(p, seed, tag, row0, x.device)
     if torch.is_grad_enabled():
         for name, t in (("weight", weight), ("bias", bias), ("scale", scale)):

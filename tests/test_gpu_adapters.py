@@ -547,3 +547,20 @@ def test_gradients_of_many_tiles_a_workgroup(tile, dtype, p):
     assert max(map(len, tiles_of_workgroups(24676, 1536))) == 3
     tile(256)
     Case(24676, 1536, 64, 8, [4000, 60, 7000, 1, 9000, 4600], [0, 1, -1, 2, 1, 0], 3, dtype, seed=12).check(p=p, seed=6, tag=3)
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "A", "B", "bias", "scale"])
+def test_forward_mode_is_refused(name):
+    """A tensor with a tangent requires no gradient; its tangent must not vanish."""
+    import torch.autograd.forward_ad as fwd
+    c = Case(70, 32, 48, 4, [30, 40], [0, 1], 2, torch.float32)
+    args = dict(x=c.x.detach(), weight=c.W, A=c.A.detach(), B=c.B.detach(), row_start=c.row_start, adapter=c.adapter, bias=c.b, scale=c.scale)
+    y = ops.adapter_linear(**args)
+    with fwd.dual_level():
+        args[name] = fwd.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(NotImplementedError, match=f"{name} carries"):
+            ops.adapter_linear(**args)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match=f"{name} carries"):
+            ops.adapter_linear(**args)
+        args[name] = fwd.unpack_dual(args[name]).primal
+        assert torch.equal(ops.adapter_linear(**args), y)                    # within a level, without a tangent

@@ -196,3 +196,17 @@ def test_a_seed_changed_before_the_backward_pass_is_an_error():
     word.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("relu", [False, True])
+def test_forward_mode_is_refused(relu):
+    """A tensor with a tangent requires no gradient; its tangent must not vanish."""
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(4, 9, device="cuda")
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="x carries"):
+            ops.dropout(d, 0.3, 5, relu=relu)
+        assert torch.equal(ops.dropout(fwd.unpack_dual(d).primal, 0.3, 5, relu=relu), ops.dropout(x, 0.3, 5, relu=relu))
+    with pytest.raises(NotImplementedError, match="x carries"):
+        torch.func.jvp(lambda t: ops.dropout(t, 0.3, 5, relu=relu), (x,), (x,))

@@ -158,3 +158,20 @@ def test_a_leaf_of_another_stream_is_refused_within_a_capture(monkeypatch):
     h = torch.zeros(3, requires_grad=True) * 1
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     ops._of_one_stream(h * 2, 1), ops._of_one_stream(h * 2, 2)                # no leaf: its nodes are not looked at
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    x, v = torch.ones(3), torch.full((3,), 2.0)
+    ops._no_tangents(x=x, bias=None)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, v)
+        assert not d.requires_grad                                           # why nothing else would notice
+        ops._no_tangents(x=x, bias=None)
+        with pytest.raises(NotImplementedError, match="bias carries"):
+            ops._no_tangents(x=x, bias=d)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="x carries"):
+            ops._no_tangents(x=d)
+    with pytest.raises(NotImplementedError, match="x carries"):
+        torch.func.jvp(lambda t: (ops._no_tangents(x=t), t * 2)[1], (x,), (v,))
+    ops._no_tangents(x=x)
