@@ -256,7 +256,16 @@ __global__ __launch_bounds__(64 * NW) void k_shrink(const T* __restrict__ X, lon
   }
 }
 
-// the same for requests of few rows (single tokens): a wave takes one row and four ranks, its lanes the reduction
+// A launch takes fewer than 2^32 threads along one dimension of its grid: what may come to more is laid out over y too.
+constexpr long long GRID_X = 1 << 22;
+inline dim3 grid_of(long long blocks) {
+  const long long x = blocks < GRID_X ? blocks : GRID_X;
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+// number of this workgroup in such a grid; the last ones lie past the blocks asked for
+__device__ __forceinline__ long long block_of_grid() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+
+// t / u for requests of few rows (single tokens): a wave takes one row and four ranks, its lanes the reduction
 constexpr int SR_RANKS = 4;
 
 template <typename T, bool DROP>
@@ -264,7 +273,7 @@ __global__ __launch_bounds__(256) void k_shrink_rows(const T* __restrict__ X, lo
                                                      long long stride_a, int rank, float factor, Segs sg, KeepArgs ka,
                                                      float* __restrict__ t, int ldt) {
   const int lane = threadIdx.x & 63, groups = ldt / SR_RANKS;
-  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long id = block_of_grid() * 4 + (threadIdx.x >> 6);
   const int row = (int)(id / groups), i0 = (int)(id % groups) * SR_RANKS;
   if (row >= sg.M) return;
   const int q = seg_find(sg, row);
@@ -1610,7 +1619,7 @@ int shrink(const hm_adapter_args& g, const T* X, long long ldx, int K, const T* 
   const float f = drop ? ka.up : 1.f;
   if (few_rows_each(g)) {
     const long long waves = g.rows * (pad8(g.rank) / SR_RANKS);
-    const dim3 grid((unsigned)((waves + 3) / 4));
+    const dim3 grid = grid_of((waves + 3) / 4);
     if (drop) hipLaunchKernelGGL((k_shrink_rows<T, true>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t, pad8(g.rank));
     else hipLaunchKernelGGL((k_shrink_rows<T, false>), grid, dim3(256), 0, st, X, ldx, K, R, ldr, stride_a, g.rank, f, sg, ka, t, pad8(g.rank));
   } else {

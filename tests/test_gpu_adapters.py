@@ -564,3 +564,31 @@ def test_forward_mode_is_refused(name):
             ops.adapter_linear(**args)
         args[name] = fwd.unpack_dual(args[name]).primal
         assert torch.equal(ops.adapter_linear(**args), y)                    # within a level, without a tangent
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_single_rows_than_one_dimension_of_a_grid(dtype):
+    """Single rows times ranks over 2^28: 2^24 workgroups of 256 threads, 2^32 threads along one dimension, are refused by a launch.
+    y and dx in 64 bits on the GPU."""
+    rows, k, n, r, na = (1 << 20) + 64, 8, 8, 256, 3
+    c = Case(rows, k, n, r, [], [], na, dtype, seed=21)
+    c.row_start = torch.arange(rows + 1, dtype=torch.int32, device="cuda")
+    c.adapter = torch.arange(rows, dtype=torch.int32, device="cuda") % (na + 1) - 1
+    for v in (c.A, c.B):
+        v.requires_grad_(False)                        # (sums over a million requests of one row are another matter)
+    y = c.call()
+    (dx,) = torch.autograd.grad(y, c.x, c.dy)
+    which = c.adapter.long()
+    f = torch.finfo(dtype)
+    split = 0.0 if dtype == torch.float32 else 2.0 ** -16
+    out = {}
+    for size in (False, True):
+        d = (lambda v: v.detach().double().abs()) if size else (lambda v: v.detach().double())
+        W, s = d(c.W), d(c.scale)
+        low = torch.stack([torch.zeros_like(W)] + [s[i] * (d(c.B[i]) @ d(c.A[i])) for i in range(na)])      # (n, k) of each adapter
+        full = (W + low)[which + 1]
+        out[size] = ((full * d(c.x)[:, None, :]).sum(2) + d(c.b), (full * d(c.dy)[:, :, None]).sum(1))
+    for got, want, size, count in zip((y, dx), out[False], out[True], (k + 2 * r, n + 2 * r)):
+        tol = ((count + 8) * 2.0 ** -23 + split) * size + f.eps / 2 * want.abs() + f.smallest_normal * f.eps
+        err = (got.detach().double() - want).abs()
+        assert bool((err <= tol).all()), float((err / tol).max())
