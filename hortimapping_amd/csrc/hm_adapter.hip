@@ -1502,14 +1502,16 @@ struct Turn {
   long long ldo, so;
   int first, across, down; // first workgroup of the job, workgroups along the columns and the rows
 };
-struct Turns { Turn job[3]; int n; };
+struct Turns { Turn job[3]; int n, blocks; };
 
 template <typename T> __global__ __launch_bounds__(256) void k_turn(Turns all) {
   __shared__ T tile[64][66];
+  const long long block = block_of_grid();
+  if (block >= all.blocks) return;
   int at = 0;
-  while (at + 1 < all.n && (int)blockIdx.x >= all.job[at + 1].first) ++at;
+  while (at + 1 < all.n && (int)block >= all.job[at + 1].first) ++at;
   const Turn& jb = all.job[at];
-  const int id = blockIdx.x - jb.first, bx = id % jb.across, by = id / jb.across % jb.down, z = id / (jb.across * jb.down);
+  const int id = (int)block - jb.first, bx = id % jb.across, by = id / jb.across % jb.down, z = id / (jb.across * jb.down);
   const T* i = static_cast<const T*>(jb.in) + z * jb.si;
   T* o = static_cast<T*>(jb.out) + z * jb.so;
   const int c0 = bx * 64, r0 = by * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;    // eight values a thread
@@ -1714,11 +1716,11 @@ template <typename T> int forward(const hm_adapter_args& g, const KeepArgs& ka, 
   return project<T>(g, X, g.ld_x, g.k, W, g.ld_w, g.n, bias, lr, false, ka, y, ld_y, st);
 }
 
-void add_turn(Turns* all, int* blocks, const void* in, long long ldi, long long si, int rows, int cols, void* out, long long ldo,
+void add_turn(Turns* all, const void* in, long long ldi, long long si, int rows, int cols, void* out, long long ldo,
               long long so, int count) {
-  const Turn t = {in, ldi, si, rows, cols, out, ldo, so, *blocks, (cols + 63) / 64, (int)((ldo + 63) / 64)};
+  const Turn t = {in, ldi, si, rows, cols, out, ldo, so, all->blocks, (cols + 63) / 64, (int)((ldo + 63) / 64)};
   all->job[all->n++] = t;
-  *blocks += t.across * t.down * count;
+  all->blocks += t.across * t.down * count;           // at most 2^28 of the adapters' A and B each, 2^20 of the weight
 }
 
 template <typename T>
@@ -1731,12 +1733,11 @@ int backward(const hm_adapter_args& g, const KeepArgs& ka, const void* d_dy, lon
   const bool any = g.adapters > 0 && g.segments > 0 && g.rows > 0;
   const bool want_u = any && (d_dx != nullptr || d_da != nullptr), want_dx = d_dx != nullptr && g.rows > 0;
   Turns turns = {};
-  int blocks = 0;
-  if (want_u) add_turn(&turns, &blocks, g.d_b, g.rank, (long long)g.n * g.rank, g.n, g.rank, bt, p.npad, g.rank * p.npad, g.adapters);
-  if (want_dx) add_turn(&turns, &blocks, W, g.ld_w, 0, g.n, g.k, wt, p.npad, 0, 1);
-  if (want_dx && any) add_turn(&turns, &blocks, g.d_a, g.k, (long long)g.rank * g.k, g.rank, g.k, at, p.rpad, g.k * p.rpad, g.adapters);
+  if (want_u) add_turn(&turns, g.d_b, g.rank, (long long)g.n * g.rank, g.n, g.rank, bt, p.npad, g.rank * p.npad, g.adapters);
+  if (want_dx) add_turn(&turns, W, g.ld_w, 0, g.n, g.k, wt, p.npad, 0, 1);
+  if (want_dx && any) add_turn(&turns, g.d_a, g.k, (long long)g.rank * g.k, g.rank, g.k, at, p.rpad, g.k * p.rpad, g.adapters);
   if (turns.n > 0) {
-    hipLaunchKernelGGL((k_turn<T>), dim3(blocks), dim3(256), 0, st, turns);
+    hipLaunchKernelGGL((k_turn<T>), grid_of(turns.blocks), dim3(256), 0, st, turns);
     HM_CHECK_HIP(hipGetLastError());
   }
   int rc;

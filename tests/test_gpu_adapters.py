@@ -592,3 +592,24 @@ def test_more_single_rows_than_one_dimension_of_a_grid(dtype):
         tol = ((count + 8) * 2.0 ** -23 + split) * size + f.eps / 2 * want.abs() + f.smallest_normal * f.eps
         err = (got.detach().double() - want).abs()
         assert bool((err <= tol).all()), float((err / tol).max())
+
+
+def test_transposes_of_more_adapters_than_one_dimension_of_a_grid():
+    """65535 adapters of 16384 columns: 65535 x 257 workgroups transpose A and B.  dx of the rows, in 64 bits on the GPU."""
+    na, k, n, rows, dtype = 65535, 16384, 8, 24, torch.bfloat16
+    c = Case(rows, k, n, 1, [1] * rows, [0, na - 1, -1] + [(i * 7919) % na for i in range(rows - 3)], 1, dtype, seed=22)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    c.A = torch.empty(na, 1, k, dtype=dtype, device="cuda").normal_(generator=g).mul_(k ** -0.5)
+    c.B = torch.empty(na, n, 1, dtype=dtype, device="cuda").normal_(generator=g)
+    c.scale = None
+    (dx,) = torch.autograd.grad(c.call(), c.x, c.dy)
+    f = torch.finfo(dtype)
+    out = {}
+    for size in (False, True):
+        d = (lambda v: v.detach().double().abs()) if size else (lambda v: v.detach().double())
+        a = c.adapter.long().clamp_min(0)
+        u = (d(c.dy) * d(c.B[a][:, :, 0])).sum(1, keepdim=True) * (c.adapter >= 0)[:, None]
+        out[size] = d(c.dy) @ d(c.W) + u * d(c.A[a][:, 0])
+    tol = ((n + 2 + 8) * 2.0 ** -23 + 2.0 ** -16) * out[True] + f.eps / 2 * out[False].abs() + f.smallest_normal * f.eps
+    err = (dx.double() - out[False]).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
