@@ -118,10 +118,11 @@ template <typename T>
 int launch(int kind, const void* in, long long ld_in, const void* y, long long ld_y, void* out, long long ld_out,
            long long rows, int cols, const KeepArgs& ka, hipStream_t st) {
   const uint32_t nb = (uint32_t)((cols + 7ll) / 8);
-  const long long n_blocks = rows * nb;
+  // a launch takes fewer than 2^32 threads along a dimension; rows of whole blocks would come to that at 274 GB of 16-bit values
+  constexpr long long per = DR_THREADS * DR_PER, most = 0xffffffffll / DR_THREADS * per;
+  if (rows > most / nb) { hm_set_error("hm_dropout: %lld x %d values are too many for one call", rows, cols); return -1; }
+  const long long n_blocks = rows * nb, grid = (n_blocks + per - 1) / per;
   const RowDiv rd = {nb, nb == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / nb)};
-  const long long per = DR_THREADS * DR_PER, grid = (n_blocks + per - 1) / per;
-  if (grid > 0x7fffffffll) { hm_set_error("hm_dropout: %lld x %d values are too many for one call", rows, cols); return -1; }
   const T *i = static_cast<const T*>(in), *v = static_cast<const T*>(y);
   T* o = static_cast<T*>(out);
 #define HM_GO(KIND) hipLaunchKernelGGL((k_dropout<T, KIND>), dim3((unsigned)grid), dim3(DR_THREADS), 0, st, i, ld_in, v, ld_y, o, \

@@ -351,7 +351,8 @@ int hm_prep_box_select(const double* d_pts, int n, const double* d_boxes, int B,
  *   seed    the 64-bit seed; d_seed (or NULL): a device word added to it, read when the kernel runs -- what a replayed graph changes
  *   tag     tells streams of one seed apart (a layer's number);  row0: number of the first row (a shard, a chunk of a batch)
  * hm_dropout_backward: dx from dy.  relu != 0: from d_y, the forward's OUTPUT (0 where nothing passed; nothing is drawn);
- * relu == 0: d_y is not read, the draws are made again from the same seed, tag, row0 and p. */
+ * relu == 0: d_y is not read, the draws are made again from the same seed, tag, row0 and p.
+ * A call takes up to 2^34 - 1024 blocks of eight columns (a row's last block counts whole) and refuses more. */
 int hm_dropout(const void* d_x, long long ld_x, void* d_y, long long ld_y, long long rows, int cols, int type, int relu, double p,
                unsigned long long seed, const unsigned long long* d_seed, unsigned tag, unsigned long long row0, void* stream);
 int hm_dropout_backward(const void* d_dy, long long ld_dy, const void* d_y, long long ld_y, void* d_dx, long long ld_dx,

@@ -175,3 +175,14 @@ def test_forward_mode_tangents_are_refused():
     with pytest.raises(NotImplementedError, match="x carries"):
         torch.func.jvp(lambda t: (ops._no_tangents(x=t), t * 2)[1], (x,), (v,))
     ops._no_tangents(x=x)
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_dropout_of_more_values_than_a_launch_takes(kind):
+    """2^32 threads (2^31 rows of eight blocks, 1024 blocks a workgroup of 256): refused before anything is launched."""
+    lib = _lib.lib()
+    for rows in (1 << 31, (1 << 63) - 1):
+        rc = lib.hm_dropout(4096, 64, 4096, 64, rows, 64, kind, 0, 0.5, 1, None, 0, 0, None)
+        assert rc < 0 and b"too many" in lib.hm_last_error()
+        rc = lib.hm_dropout_backward(4096, 64, 4096, 64, 4096, 64, rows, 64, kind, 1, 0.5, 1, None, 0, 0, None)
+        assert rc < 0 and b"too many" in lib.hm_last_error()
