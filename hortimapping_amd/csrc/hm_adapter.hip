@@ -1668,6 +1668,20 @@ int pick_tile(long long rows, int n, int k, int size) {
 
 int g_tile = 0;            // hm_debug_set_adapter_tile
 
+template <typename T> int tile_of(long long rows, int Nn, int Kk) {
+  if (g_tile != 0 && (g_tile != WIDE || Kk >= Lines<T>::KB)) return g_tile == 128 && sizeof(T) == 4 ? 64 : g_tile;
+  return pick_tile(rows, Nn, Kk, sizeof(T));
+}
+
+// Tiles of 64 or 128 are a workgroup of 256 threads each, of which a launch takes fewer than 2^32 along a dimension: 2^36 fp32 outputs
+// (275 GB) of a short reduction come to more, and are refused before anything is launched.
+template <typename T> int check_tiles(const char* name, long long rows, int Nn, int Kk) {
+  const int tile = tile_of<T>(rows, Nn, Kk);
+  if (tile != WIDE && ((rows + tile - 1) / tile) * ((Nn + tile - 1) / tile) >= 1ll << 24) {
+    hm_set_error("%s: %lld x %d outputs are too many for one call", name, rows, Nn); return -1; }
+  return 0;
+}
+
 template <typename T>
 int project(const hm_adapter_args& g, const T* X, long long ldx, int Kk, const T* W, long long ldw, int Nn, const T* bias,
             const LowRank& lr, bool drop, const KeepArgs& ka, T* out, long long ldo, hipStream_t st) {
@@ -1675,14 +1689,13 @@ int project(const hm_adapter_args& g, const T* X, long long ldx, int Kk, const T
 #define HM_GO(BM, BN, WGM, WGN, D)                                                                                                   \
   hipLaunchKernelGGL((k_project<T, BM, BN, WGM, WGN, D>), dim3((unsigned)(((g.rows + BM - 1) / BM) * ((Nn + BN - 1) / BN))),         \
                      dim3(64 * WGM * WGN), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, (Nn + BN - 1) / BN)
-  int tile = pick_tile(g.rows, Nn, Kk, sizeof(T));
-  if (g_tile != 0 && (g_tile != WIDE || Kk >= Lines<T>::KB)) tile = g_tile;
-  if (tile == 256) {
+  const int tile = tile_of<T>(g.rows, Nn, Kk);
+  if (tile == WIDE) {
     const int tm = (int)((g.rows + WIDE - 1) / WIDE), tn = (Nn + WIDE - 1) / WIDE;
     const dim3 grid((long long)tm * tn < 256 ? tm * tn : 256);
     if (drop) hipLaunchKernelGGL((k_project_wide<T, true>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, tm, tn);
     else hipLaunchKernelGGL((k_project_wide<T, false>), grid, dim3(256), 0, st, X, ldx, Kk, W, ldw, Nn, bias, lr, sg, ka, out, ldo, tm, tn);
-  } else if (tile == 128 && sizeof(T) == 2) {
+  } else if (tile == 128) {
     if constexpr (sizeof(T) == 2) { if (drop) HM_GO(128, 128, 2, 2, true); else HM_GO(128, 128, 2, 2, false); }
   } else {
     if (drop) HM_GO(64, 64, 2, 2, true); else HM_GO(64, 64, 2, 2, false);
@@ -1696,13 +1709,14 @@ template <typename T> int forward(const hm_adapter_args& g, const KeepArgs& ka, 
   const T *X = static_cast<const T*>(g.d_x), *W = static_cast<const T*>(g.d_w), *A = static_cast<const T*>(g.d_a);
   const T* bias = static_cast<const T*>(g.d_bias);
   T* y = static_cast<T*>(d_y);
-  const bool any = g.adapters > 0 && g.segments > 0;
+  const bool any = g.adapters > 0 && g.segments > 0, few = g.rows <= FEW_ROWS && g_tile == 0;
+  if (!few && check_tiles<T>("hm_adapter_linear", g.rows, g.n, g.k)) return -1;
   if (any) {
     const int rc = shrink<T>(g, X, g.ld_x, g.k, A, g.k, (long long)g.rank * g.k, ka.threshold != 0, ka, d_t, st);
     if (rc) return rc;
   }
   const LowRank lr = {any ? d_t : nullptr, g.d_b, (long long)g.n * g.rank, g.rank, g.rank, pad8(g.rank)};
-  if (g.rows <= FEW_ROWS && g_tile == 0) {
+  if (few) {
     const dim3 grid((g.n + 15) / 16, (unsigned)((g.rows + 63) / 64));
     const Segs sg = segs_of(g);
 #define HM_GO(MT) hipLaunchKernelGGL((k_project_few<T, MT>), grid, dim3(64 * FEW_WAVES), 0, st, X, g.ld_x, g.k, W, g.ld_w, g.n, bias, lr, sg, y, ld_y)
@@ -1732,6 +1746,7 @@ int backward(const hm_adapter_args& g, const KeepArgs& ka, const void* d_dy, lon
   float* u = reinterpret_cast<float*>(ws + p.u);
   const bool any = g.adapters > 0 && g.segments > 0 && g.rows > 0;
   const bool want_u = any && (d_dx != nullptr || d_da != nullptr), want_dx = d_dx != nullptr && g.rows > 0;
+  if (want_dx && check_tiles<T>("hm_adapter_linear_backward", g.rows, g.k, g.n)) return -1;
   Turns turns = {};
   if (want_u) add_turn(&turns, g.d_b, g.rank, (long long)g.n * g.rank, g.n, g.rank, bt, p.npad, g.rank * p.npad, g.adapters);
   if (want_dx) add_turn(&turns, W, g.ld_w, 0, g.n, g.k, wt, p.npad, 0, 1);

@@ -367,7 +367,8 @@ int hm_dropout_backward(const void* d_dy, long long ld_dy, const void* d_y, long
  * ascend gives unspecified values for the rows concerned, nothing else.
  * A row's result depends on its own row and adapter alone (not on the batch around it, bit for bit as long as the same kernels
  * run; an infinity or NaN in another request or adapter does not reach it).  An infinity among a result's own factors may come out
- * as NaN: 32-bit values are multiplied in two parts. */
+ * as NaN: 32-bit values are multiplied in two parts.
+ * 2^24 tiles of 64 x 64 outputs and more (2^36 fp32 values of y or dx) with a short reduction are refused. */
 #define HM_ADAPTER_MAX_ROWS 16777216
 #define HM_ADAPTER_MAX_WIDTH 65536
 #define HM_ADAPTER_MAX_RANK 256

@@ -186,3 +186,13 @@ def test_dropout_of_more_values_than_a_launch_takes(kind):
         assert rc < 0 and b"too many" in lib.hm_last_error()
         rc = lib.hm_dropout_backward(4096, 64, 4096, 64, 4096, 64, rows, 64, kind, 1, 0.5, 1, None, 0, 0, None)
         assert rc < 0 and b"too many" in lib.hm_last_error()
+
+
+def test_adapter_outputs_of_more_tiles_than_a_launch_takes():
+    """2^18 x 2^6 tiles of 64 x 64 outputs in fp32, of 256 threads each: refused before anything is launched."""
+    lib, rows = _lib.lib(), 1 << 24
+    a = args(rows=rows, k=16, n=4096, segments=0, ld_x=16, ld_w=16)
+    assert lib.hm_adapter_linear(ctypes.byref(a), 4096, 4096, 4096, None) < 0 and b"too many" in lib.hm_last_error()
+    a = args(rows=rows, k=4096, n=16, segments=0, ld_x=4096, ld_w=4096)
+    assert lib.hm_adapter_linear_backward(ctypes.byref(a), 4096, 16, 4096, 4096, 4096, None, None, 4096, 1 << 40, None) < 0
+    assert b"too many" in lib.hm_last_error()
