@@ -18,7 +18,10 @@ __device__ __forceinline__ float rounded_product(float a, float b) {
 __device__ __forceinline__ float dot3_third_rounded(float a0, float b0, float a1, float b1, float a2, float b2) {
   return fmaf(a0, b0, a1 * b1) + rounded_product(a2, b2);
 }
-
+// the same with the first product rounded and the others added to it by fused multiply-adds
+__device__ __forceinline__ float dot3_first_rounded(float a0, float b0, float a1, float b1, float a2, float b2) {
+  return fmaf(a2, b2, fmaf(a1, b1, rounded_product(a0, b0)));
+}
 
 constexpr int HID = 512;        // hidden width of the DeepSDF decoder (specs.json:8)
 constexpr int TQ = 64;          // decoder queries per workgroup tile (2 MFMA N-blocks of 32)

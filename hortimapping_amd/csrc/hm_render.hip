@@ -32,7 +32,7 @@ __device__ __forceinline__ float det3f(const float* M, int ld) {
 // torch.linspace(start, end, steps)[j] in fp32 (symmetric two-sided formula of ATen's CPU/CUDA kernels)
 __device__ __forceinline__ float linspace_at(float start, float end, int steps, int j) {
   const float step = (end - start) / (float)(steps - 1);
-  return (j < steps / 2) ? start + step * (float)j : end - step * (float)(steps - 1 - j);
+  return (j < steps / 2) ? fmaf(step, (float)j, start) : fmaf(-step, (float)(steps - 1 - j), end);
 }
 
 }  // namespace
@@ -50,8 +50,8 @@ __global__ void k_transform_points(const float* __restrict__ pw, int n_in_stride
     const float* T = T_ow + (size_t)b * 16;
     const float* p = pw + ((size_t)b * n_in_stride + i) * 3;
     const float x = p[0], y = p[1], z = p[2];
-    o[0] = (x * T[0] + y * T[1]) + z * T[2] + T[3];
-    o[1] = (x * T[4] + y * T[5]) + z * T[6] + T[7];
+    o[0] = hm::dot3_first_rounded(y, T[1], x, T[0], z, T[2]) + T[3];
+    o[1] = hm::dot3_first_rounded(y, T[5], x, T[4], z, T[6]) + T[7];
     o[2] = hm::dot3_third_rounded(x, T[8], y, T[9], z, T[10]) + T[11];
     o[3] = 1.f;
   }
@@ -121,9 +121,9 @@ __global__ __launch_bounds__(256) void k_sample_rays(const RenderCfg cfg, const 
     const float* dir = rb.rays + (((size_t)b * cfg.F + f) * cfg.R + r) * 3;
     const float d = linspace_at(fp[12], fp[13], cfg.M, j);                      // optimizer.py:111
     const float x = dir[0] * d, y = dir[1] * d, z = dir[2] * d;                 // loss.py:30
-    o[0] = fmaf(z, fp[2], fmaf(y, fp[1], hm::rounded_product(x, fp[0]))) + fp[3];                         // loss.py:32-33
+    o[0] = hm::dot3_first_rounded(x, fp[0], y, fp[1], z, fp[2]) + fp[3];        // loss.py:32-33
     o[1] = hm::dot3_third_rounded(x, fp[4], y, fp[5], z, fp[6]) + fp[7];
-    o[2] = (x * fp[8] + y * fp[9]) + z * fp[10] + fp[11];
+    o[2] = hm::dot3_first_rounded(y, fp[9], x, fp[8], z, fp[10]) + fp[11];
     valid = sqrtf(hm::dot3_third_rounded(o[1], o[1], o[0], o[0], o[2], o[2])) < fp[14];   // loss.py:38
     o[3] = valid ? 1.f : 0.f;
   }
