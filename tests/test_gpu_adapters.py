@@ -613,3 +613,45 @@ def test_transposes_of_more_adapters_than_one_dimension_of_a_grid():
     tol = ((n + 2 + 8) * 2.0 ** -23 + 2.0 ** -16) * out[True] + f.eps / 2 * out[False].abs() + f.smallest_normal * f.eps
     err = (dx.double() - out[False]).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("side", [64, 128, 256])
+def test_every_tile_on_odd_strides(tile, side, dtype):
+    """x, weight and dy that start between vectors and have odd row strides: the bits of contiguous ones."""
+    tile(side)
+    c = Case(700, 333, 270, 12, [100, 37, 400, 130], [0, 2, -1, 1], 3, dtype, seed=30)
+    want = c.check(p=0.2, seed=8)
+
+    def odd(t, before, behind):
+        w = torch.full((t.shape[0], t.shape[1] + before + behind), float("nan"), dtype=dtype, device="cuda")
+        w[:, before:before + t.shape[1]] = t.detach()
+        return w[:, before:before + t.shape[1]]
+    x, W = odd(c.x, 3, 5).requires_grad_(), odd(c.W, 1, 3)
+    y = ops.adapter_linear(x, W, c.A, c.B, c.row_start, c.adapter, bias=c.b, scale=c.scale, p=0.2, seed=8)
+    got = [y] + list(torch.autograd.grad(y, (x, c.A, c.B), odd(c.dy, 5, 2)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("side", [64, 128, 256])
+def test_offsets_past_32_bits(tile, side):
+    """y, and then x and dx, of more than 2^31 values: the last rows are what a call on them alone gives."""
+    rows, last, dtype = 530000, 1000, torch.bfloat16
+    assert rows * 4096 > 2 ** 31
+    tile(side)
+    for k, n in ((64, 4096), (4096, 64)):
+        c = Case(last, k, n, 8, [400, 600], [0, 1], 2, dtype, seed=31)
+        want = c.call(p=0.1, seed=3, row0=rows - last)
+        want = [want] + list(torch.autograd.grad(want, c.x, c.dy))
+        x = torch.zeros(rows, k, dtype=dtype, device="cuda")
+        x[-last:] = c.x.detach()
+        dy = torch.zeros(rows, n, dtype=dtype, device="cuda")
+        dy[-last:] = c.dy
+        c.row_start = torch.tensor([0, rows - last, rows - 600, rows], dtype=torch.int32, device="cuda")
+        c.adapter = torch.tensor([1, 0, 1], dtype=torch.int32, device="cuda")
+        c.x = x.requires_grad_()
+        whole = c.call(p=0.1, seed=3)
+        assert torch.equal(whole[-last:], want[0]) and torch.equal(whole[:2000], c.b.expand(2000, n))
+        (dx,) = torch.autograd.grad(whole, c.x, dy)
+        assert torch.equal(dx[-last:], want[1]) and not dx[:2000].any()
+        del x, dy, whole, dx, c

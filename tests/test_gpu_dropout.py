@@ -210,3 +210,19 @@ def test_forward_mode_is_refused(relu):
         assert torch.equal(ops.dropout(fwd.unpack_dual(d).primal, 0.3, 5, relu=relu), ops.dropout(x, 0.3, 5, relu=relu))
     with pytest.raises(NotImplementedError, match="x carries"):
         torch.func.jvp(lambda t: ops.dropout(t, 0.3, 5, relu=relu), (x,), (x,))
+
+
+@pytest.mark.parametrize("relu", [False, True])
+def test_offsets_past_32_bits(relu):
+    """More than 2^31 values: the last rows are what a call on them alone gives."""
+    rows, cols, last = 530000, 4099, 300
+    assert rows * 4096 > 2 ** 31
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[-last:] = data(last, cols, torch.bfloat16)
+    part = x[-last:].clone().requires_grad_()
+    x.requires_grad_()
+    y, z = ops.dropout(x, 0.3, 11, tag=2, relu=relu), ops.dropout(part, 0.3, 11, tag=2, row0=rows - last, relu=relu)
+    assert torch.equal(y[-last:], z) and not y[:1000].any() and bool(z.any())
+    dy = torch.ones_like(x)
+    (dx,), (dz,) = torch.autograd.grad(y, x, dy), torch.autograd.grad(z, part, dy[-last:])
+    assert torch.equal(dx[-last:], dz) and bool(dz.any())
