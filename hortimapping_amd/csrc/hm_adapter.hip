@@ -210,7 +210,7 @@ __device__ __forceinline__ void strip_sum(f32x4 (&acc)[BT][AT], const T* A, long
 }
 
 // ---- t / u: 32 rows x up to 64 ranks a workgroup, its waves share the reduction.  Bound by reading X once: 131072 x 512 bf16 in
-// 25 us (5.3 TB/s), 65536 x 512 fp32 in 28 (4.9 TB/s); rows of 259 values, which start between lines, 35 us.
+// 25 us (5.3 TB/s), 65536 x 512 fp32 in 27 (5.0 TB/s); rows of 259 values, which start between lines, 34 us.
 constexpr int SH_ROWS = 32, SH_RANKS = 64;
 
 template <typename T, int RT, int NW, bool DROP>
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(256) void k_shrink_rows(const T* __restrict__ X, lo
 // ---- the projection with the low-rank part: out (M, Nn) = X (M, Kk) W^T (+ bias) + t Bt_a^T, tiles of BM x BN in LDS, rows of
 // 128 bytes along the reduction, 16-byte chunks XOR-ed with the row (conflict-free 16-byte reads).  Two LDS buffers and one
 // barrier a step: the step after next is on its way to registers while a step is computed.  Bound by the two workgroups a CU that
-// its registers allow, neither of which hides all waits of the other: 6001 x 1024 x 4096 fp16 with rank 32 96 us (524 TFLOP/s).
+// its registers allow, neither of which hides all waits of the other: 6001 x 1024 x 4096 fp16 with rank 32 97 us (519 TFLOP/s).
 __device__ __forceinline__ f32x16 mma32(uint4 a, uint4 b, f32x16 c, f16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
@@ -694,8 +694,9 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void k_project(const T* __restri
 // buffer and sends for the step after that; one barrier a step, behind which the next step's first fragments are read.  128 x 128
 // outputs a wave need half an LDS byte for each that 128 x 64 need three quarters of.  Loads run on across tiles: a new tile's
 // first steps are under way while the last one is finished and stored.
-// Measured without adapters: 8192 x 4096 x 4096 bf16 236 us (1165 TFLOP/s), 131072 x 512 x 512 bf16 98 us (half of it the way in and
-// out of 512 tiles), 65536 x 512 x 512 fp32 297 us (116 TFLOP/s); rank 64 on the first of these: 287 us.
+// Measured without adapters: 8192 x 4096 x 4096 bf16 243 us (1131 TFLOP/s), 131072 x 512 x 512 bf16 89 us (half of it the way in and
+// out of 1024 tiles), 65536 x 512 x 512 fp32 302 us (114 TFLOP/s).  With them: the first at rank 64 278 us, the last at rank 16 302 us
+// where requests end with tiles and 339 where they end anywhere (rows of several requests are finished block by block).
 constexpr int WIDE = 256, LDS_REQUESTS = 256;
 
 // The sums of the wide projection, by the names of their registers: block (n, m) of a wave is a[16 (4 n + m)] .. + 15, all 256
@@ -1105,8 +1106,9 @@ __global__ __launch_bounds__(256, 1) void k_project_wide(const T* __restrict__ X
 }
 
 // ---- few rows: the weights are read once for each 64 rows, sixteen outputs a workgroup, its waves share the reduction
-// (up to 256 rows: 45 us of 256 rows x 4096 x 4096 against 60 of the tiles of 64, 29 against 59 of 128 rows; 64 rows bf16 with
-// 48 adapters of rank 16 12.7 us, bound by the way of W through the LDS, 2.7 TB/s)
+// (up to 256 rows: 37 us of 256 rows x 4096 x 4096 bf16 against 56 of the tiles of 64, 21 against 54 of 128 rows; 64 rows with
+// 48 adapters of rank 16 13 us, bound by the way of W through the LDS, 2.6 TB/s).  Forward alone: dx of few rows takes the tiles of
+// 64, which have the mask of x (54 of the 317 us of a training call of 128 single rows x 4096 x 4096).
 constexpr int FEW_ROWS = 256, FEW_WAVES = 8;
 
 template <typename T, int MT>
@@ -1176,8 +1178,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_project_few(const T* __restr
 //   16 bit  32 rows a wave and step (eight a lane), turned 8 x 8 in registers, 16 x 16 x 32 bf16 products with t split in two
 //           (an eighth of the matrix time of the fp32 products, which bounded ranks over 16).
 // About 1024 workgroups, each a run of rows; partial sums of (run, request) pairs in slots, added in order by k_outer_sum.  Bound by the
-// time that loads take to come back: 2.6 TB/s over x and dy of 131072 rows (79 us).  The next step's loads sent ahead of this one's
-// products cost the registers of a third workgroup a CU and take 92 us; four workgroups a CU spill.
+// time that loads take to come back: 2.7 TB/s over x and dy of 131072 rows (76 us).  The next step's loads sent ahead of this one's
+// products cost the registers of a third workgroup a CU and take 92 us; four workgroups a CU spill.  Requests of one row each are
+// taken one after the other, with one wave at work: 202 us of 128 rows x (4096 + 4096).
 constexpr int OU_COLS = 128;
 
 template <typename T, int RT> struct OuterSum {
@@ -1640,12 +1643,17 @@ int shrink(const hm_adapter_args& g, const T* X, long long ldx, int K, const T* 
 }
 
 // Outputs a side of a workgroup's tile: 256 (k_project_wide: whole rounds of one workgroup a CU count, the last one is as long as the
-// others), 128 (two a CU) or 64 (five).  By the time that rounds of each took on an MI355X, in us, with s steps of 128 bytes along the
-// reduction (rank 16):
+// others), 128 (two a CU) or 64 (five).  By the time that a round of each takes, in us, with s steps of 128 bytes along the reduction:
 //   16 bits  wide 14 + 1.67 s a round of 256 tiles, 128: 4.7 + 1.29 s a round of 512; 64 where those of 128 would not fill the CUs once
 //            (512 x 4096 x 4096: 49 against 60) or half of each would lie beside the outputs
 //   fp32     wide 38 + 6.8 s a round, 64: 2.97 s a round of 1280 (128 takes as long from 2048 rows of 512 on, twice as long below)
-// e.g. 131072 x 512 x 512 bf16 wide 117, 128: 149, 64: 174; 52000 rows 76, 62, 69; 8192 x 4096 x 4096 256, 378, 616.
+// The rule knows neither the rank nor where requests end, so it tells the sides apart rather than the time.  Kernel times of sides
+// 256 / 128 / 64 (fp32: 256 / 64) with requests of equal lengths, and what the rule says of the two that it compares:
+//   131072 x 512 x 512 bf16 rank 8    96 / 115 / 143 (109, 122)     8192 x 4096 x 4096 bf16 rank 64  278 / 386 / 598 (242, 351)
+//   131072 x 512 x 259 bf16 rank 8    93 /  96 /  96 (109,  92)     6001 x 1024 x 4096 fp16 rank 32  106 /  97 / 127 ( 81,  76)
+//    65536 x 512 x 253 fp16 rank 16   35 /  40 /  48 ( 27,  32)    52000 x 512 x 512 bf16 rank 16     60 /  52 /  60 ( 55,  50)
+//    65536 x 512 x 512 fp32 rank 16  302 / 320       (294, 309)    32768 x 512 x 512 fp32 rank 4     141 / 155       (147, 157)
+// Requests that end inside tiles cost the wide tile most: 65536 x 512 x 253 takes 55 us then, 65536 x 512 x 512 fp32 339.
 int pick_tile(long long rows, int n, int k, int size) {
   auto tiles = [&](int t) { return ((rows + t - 1) / t) * ((n + t - 1) / t); };
   const int line = 128 / size;

@@ -9,9 +9,11 @@
 // One thread takes one block of eight columns (one generator call), so a row of any length starts its own blocks; odd rows
 // (253 columns) are read at the alignment they have, the last block of a row in pieces of 4, 2 and 1.
 //
-// Bound by memory: 131072 x 512 fp32 forward 97 us (5.5 TB/s), ReLU backward 149 us (5.4 TB/s); 32768 x 512 fp16 14.5 us (4.6).
-// 131072 x 253 bf16, every row at another alignment: 37 and 47 us (3.6 and 4.2 TB/s).  A generator call's ten rounds hide behind
-// the loads: four blocks a thread (DR_PER) keep enough of these in flight.
+// Bound by memory: 131072 x 512 fp32 with ReLU forward 97 us (5.5 TB/s), backward 149 us (5.4 TB/s), without ReLU 101 us either way
+// (5.3); 32768 x 512 fp16 15 us (4.5).  131072 x 253 bf16, every row at another alignment: 31 to 37 us forward, 35 to 48 us
+// backward with ReLU (on different cards), 30 us either way without.  (Contiguous tensors whose backward pass draws nothing could be
+// taken as one long row, every access aligned; they are not.)  A generator call's ten rounds hide behind the loads: four blocks a
+// thread (DR_PER) keep enough of these in flight.
 #include "hm_internal.h"
 #include "hm_keep.h"
 #include "../../include/hortimapping_amd.h"
