@@ -259,7 +259,8 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, A: torch.Tensor, B: to
     rows row_start[q] .. row_start[q + 1] - 1 (int32, ascending, S + 1 of them) and uses adapter[q] (int32, S); a value
     outside 0 .. adapters - 1, and rows of no request, get the bare projection.  Both are read on the GPU, when the kernels
     run: a captured graph may be replayed with others.  (Before a capture with a backward pass, drop the results of eager
-    calls with the same leaves: beside a living one the call is refused.)  p, seed, tag, row0: dropout on the adapters' input, the mask of
+    calls with the same leaves: beside a living one the call is refused, which sees leaves that are handed to both calls
+    themselves, not those behind another operation.)  p, seed, tag, row0: dropout on the adapters' input, the mask of
     `dropout(x, p, seed, tag=tag, row0=row0)`.  Ranks up to 256, K and N up to 65536.
     Gradients are those of reverse mode, once; tensors with a forward-mode tangent are refused."""
     _check_float("x", x)
